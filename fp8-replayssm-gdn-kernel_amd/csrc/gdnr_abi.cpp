@@ -11,6 +11,7 @@
 
 #include <initializer_list>
 #include <string>
+#include <utility>
 
 #include "gdnr.h"
 #include "gdnr_internal.h"
@@ -1295,6 +1296,280 @@ int gdnr_dequantize_checkpoint(const gdnr_tensor* payload, const gdnr_tensor* sc
   GDNR_TRY(check_format(state, payload, scale, nullptr, granularity, tile_size, &f));
   if ((int64_t)f.B * f.HV * f.V * f.K == 0) return GDNR_OK;
   return hip_status(gdnr::launch_format_dequantize(f, stream));
+}
+
+namespace {
+// rows, sequences and heads the sequence operators' grids and 32-bit counts hold
+constexpr int64_t kMaxTokens = 1 << 23, kMaxSequences = 65535;
+
+int check_tokens(int64_t T, int64_t N) {
+  if (T > kMaxTokens) return fail(GDNR_ERR_UNSUPPORTED, "%lld tokens exceed %lld", (long long)T, (long long)kMaxTokens);
+  if (N > kMaxSequences) return fail(GDNR_ERR_UNSUPPORTED, "%lld sequences exceed %lld", (long long)N, (long long)kMaxSequences);
+  return GDNR_OK;
+}
+
+// cu_seqlens [N + 1] int32
+int check_starts(const gdnr_tensor* cu, int64_t* N) {
+  GDNR_TRY(check_desc(cu, "cu_seqlens", 1));
+  GDNR_TRY(check_dtype(cu, "cu_seqlens", {GDNR_DTYPE_I32}));
+  if (cu->shape[0] < 1) return fail(GDNR_ERR_INVALID_ARGUMENT, "cu_seqlens: empty (expected sequences + 1 offsets)");
+  *N = cu->shape[0] - 1;
+  return GDNR_OK;
+}
+
+int check_workspace(const gdnr_tensor* w, int64_t need) {
+  if (need == 0) return GDNR_OK;
+  GDNR_TRY(check_desc(w, "workspace", 1));
+  GDNR_TRY(check_dtype(w, "workspace", {GDNR_DTYPE_U8}));
+  GDNR_TRY(check_align(w, "workspace", 16));
+  if (w->shape[0] < need || w->strides[0] != 1)
+    return fail(GDNR_ERR_INVALID_ARGUMENT, "workspace: %lld contiguous bytes needed, got %lld", (long long)need,
+                (long long)w->shape[0]);
+  return GDNR_OK;
+}
+
+bool is_act16(int dt) { return dt == GDNR_DTYPE_BF16 || dt == GDNR_DTYPE_F16; }
+
+int check_head_dim(int64_t D) {
+  if (D == 64 || D == 128 || D == 256) return GDNR_OK;
+  return fail(GDNR_ERR_UNSUPPORTED, "head dim %lld: 64, 128 and 256 are built", (long long)D);
+}
+
+// [pages, page, heads, D]: a key or value cache, whose rows are found in
+// 32-bit counts of 16 bytes
+int check_cache(const gdnr_tensor* c, const char* name, int act, int64_t heads, int64_t D) {
+  GDNR_TRY(check_desc(c, name, 4));
+  GDNR_TRY(check_act_tensor(c, name, 4, {c->shape[0], c->shape[1], heads, D}, act, 16));
+  const int64_t pages = c->shape[0], page = c->shape[1];
+  if (page < 1) return fail(GDNR_ERR_INVALID_ARGUMENT, "%s: pages of no tokens", name);
+  if (pages > INT32_MAX || page > INT32_MAX || (pages && pages * page > ((int64_t)1 << 31) - 1))
+    return fail(GDNR_ERR_UNSUPPORTED, "%s: %lld pages of %lld tokens pass 2^31 slots", name, (long long)pages, (long long)page);
+  if (pages * c->strides[0] + page * c->strides[1] + heads * c->strides[2] >= ((int64_t)1 << 35))
+    return fail(GDNR_ERR_UNSUPPORTED, "%s: spans 2^36 bytes or more", name);
+  return GDNR_OK;
+}
+
+// Keys a workgroup of the attention walks, and how many such pieces the
+// longest context has. A context is cut while the launch has fewer than four
+// workgroups a compute unit, into whole steps of its four waves (128 keys), at
+// least 256 keys: a shorter piece costs as much to join as to walk.
+void attention_pieces(int64_t T, int64_t N, int64_t HQ, int64_t HKV, int64_t max_context, int32_t* piece, int32_t* pieces) {
+  const int64_t G = HQ / HKV, gt = G < 16 ? G : 16, groups = (T / (16 / gt) + N) * HKV * ((G + 15) / 16);
+  const int64_t want = 4 * (int64_t)gdnr::device_cus();
+  int64_t p = max_context;
+  if (groups < want) p = (max_context * groups + want - 1) / want;
+  p = (p + 127) / 128 * 128;
+  if (p < 256) p = 256;
+  *piece = (int32_t)(p < INT32_MAX ? p : INT32_MAX);
+  *pieces = max_context ? (int32_t)((max_context + p - 1) / p) : 1;
+}
+int64_t attention_workspace(int64_t T, int64_t HQ, int64_t D, int32_t pieces) {
+  return pieces > 1 ? (int64_t)pieces * T * HQ * (D + 2) * 4 : 0;
+}
+}  // namespace
+
+int64_t gdnr_prefill_workspace(int64_t tokens, int64_t sequences, int32_t heads, int32_t value_heads, int32_t value_dim,
+                               int32_t act_dtype, int32_t state_dtype) {
+  (void)heads, (void)value_heads, (void)value_dim, (void)act_dtype, (void)state_dtype;
+  g_last_error.clear();
+  if (tokens < 0 || sequences < 0) {
+    fail(GDNR_ERR_INVALID_ARGUMENT, "tokens and sequences must not be negative");
+    return -1;
+  }
+  return 0;
+}
+
+int gdnr_prefill(const gdnr_tensor* mixed_qkv, const gdnr_tensor* a, const gdnr_tensor* b, const gdnr_tensor* a_log,
+                 const gdnr_tensor* dt_bias, const gdnr_tensor* state, const gdnr_tensor* state_indices,
+                 const gdnr_tensor* cu_seqlens, const gdnr_tensor* has_initial_state, const gdnr_tensor* out,
+                 const gdnr_tensor* workspace, float scale, void* stream) {
+  g_last_error.clear();
+  if (!(scale - scale == 0.0f)) return fail(GDNR_ERR_INVALID_ARGUMENT, "scale: %g is not finite", (double)scale);
+  GDNR_TRY(check_desc(state, "state", 4));
+  GDNR_TRY(check_dtype(state, "state", {GDNR_DTYPE_BF16, GDNR_DTYPE_F16, GDNR_DTYPE_F32}));
+  const int64_t S = state->shape[0], HV = state->shape[1], V = state->shape[2], K = state->shape[3];
+  if (K != gdnr::kKeyDim)
+    return fail(GDNR_ERR_UNSUPPORTED, "state: K=%lld (only K=%d is built)", (long long)K, gdnr::kKeyDim);
+  if (V % gdnr::kVBlock)
+    return fail(GDNR_ERR_UNSUPPORTED, "state: V=%lld is not a multiple of %d", (long long)V, gdnr::kVBlock);
+  if (S < 1) return fail(GDNR_ERR_INVALID_ARGUMENT, "state holds no slot (slot 0 is the null slot)");
+  GDNR_TRY(check_inner_unit(state, "state"));
+  GDNR_TRY(check_align(state, "state", 16));
+  GDNR_TRY(check_desc(mixed_qkv, "mixed_qkv", 2));
+  const int act = mixed_qkv->dtype;
+  if (!is_act(act)) return fail(GDNR_ERR_INVALID_ARGUMENT, "mixed_qkv: dtype %s is not bf16|f16|f32", dtype_name(act));
+  const int64_t T = mixed_qkv->shape[0], width = mixed_qkv->shape[1], hk2 = width - HV * V;
+  if (hk2 <= 0 || hk2 % (2 * K))
+    return fail(GDNR_ERR_INVALID_ARGUMENT, "mixed_qkv: width %lld is not 2 H K + HV V (HV=%lld, V=%lld, K=%lld)",
+                (long long)width, (long long)HV, (long long)V, (long long)K);
+  const int64_t H = hk2 / (2 * K);
+  if (HV % H)
+    return fail(GDNR_ERR_INVALID_ARGUMENT, "%lld key heads do not divide %lld value heads", (long long)H, (long long)HV);
+  GDNR_TRY(check_inner_unit(mixed_qkv, "mixed_qkv"));
+  GDNR_TRY(check_align(mixed_qkv, "mixed_qkv", 16));
+  GDNR_TRY(check_desc(a, "a", 2));
+  GDNR_TRY(check_desc(b, "b", 2));
+  if (a->dtype != b->dtype || (a->dtype != act && a->dtype != GDNR_DTYPE_F32))
+    return fail(GDNR_ERR_INVALID_ARGUMENT, "a/b: dtypes %s/%s (expected both f32 or both %s)", dtype_name(a->dtype),
+                dtype_name(b->dtype), dtype_name(act));
+  GDNR_TRY(check_shape(a, "a", {T, HV}));
+  GDNR_TRY(check_shape(b, "b", {T, HV}));
+  GDNR_TRY(check_desc(a_log, "a_log", 1));
+  GDNR_TRY(check_desc(dt_bias, "dt_bias", 1));
+  GDNR_TRY(check_dtype(a_log, "a_log", {GDNR_DTYPE_F32}));
+  GDNR_TRY(check_dtype(dt_bias, "dt_bias", {GDNR_DTYPE_F32}));
+  GDNR_TRY(check_shape(a_log, "a_log", {HV}));
+  GDNR_TRY(check_shape(dt_bias, "dt_bias", {HV}));
+  int64_t N;
+  GDNR_TRY(check_starts(cu_seqlens, &N));
+  GDNR_TRY(check_index_vec(state_indices, "state_indices", N, false));
+  if (has_initial_state) GDNR_TRY(check_index_vec(has_initial_state, "has_initial_state", N, true));
+  GDNR_TRY(check_desc(out, "out", 3));
+  GDNR_TRY(check_act_tensor(out, "out", 3, {T, HV, V}, act, 16));
+  GDNR_TRY(check_tokens(T, N));
+  if (HV * V > INT32_MAX / 4 || S > INT32_MAX) return fail(GDNR_ERR_UNSUPPORTED, "state extents too large");
+  if (N * HV * V == 0) return GDNR_OK;
+  GDNR_TRY(check_workspace(workspace, gdnr_prefill_workspace(T, N, (int32_t)H, (int32_t)HV, (int32_t)V, act, state->dtype)));
+  gdnr::PrefillArgs r = {};
+  r.mixed = mixed_qkv->data, r.mx_t = mixed_qkv->strides[0];
+  r.a = a->data, r.a_t = a->strides[0], r.a_h = a->strides[1];
+  r.bgate = b->data, r.bg_t = b->strides[0], r.bg_h = b->strides[1];
+  r.a_log = (const float*)a_log->data, r.al_s = a_log->strides[0];
+  r.dt_bias = (const float*)dt_bias->data, r.db_s = dt_bias->strides[0];
+  r.state = state->data, r.st_s = state->strides[0], r.st_h = state->strides[1], r.st_v = state->strides[2];
+  r.slot = (const int32_t*)state_indices->data, r.sl_s = state_indices->strides[0], r.n_slots = (int32_t)S;
+  r.cu = (const int32_t*)cu_seqlens->data, r.cu_s = cu_seqlens->strides[0];
+  if (has_initial_state) r.started = (const uint8_t*)has_initial_state->data, r.sd_s = has_initial_state->strides[0];
+  r.out = out->data, r.o_t = out->strides[0], r.o_h = out->strides[1];
+  r.T = (int32_t)T, r.N = (int32_t)N, r.H = (int32_t)H, r.HV = (int32_t)HV, r.V = (int32_t)V, r.G = (int32_t)(HV / H);
+  r.out_scale = scale;
+  return hip_status(gdnr::launch_prefill(r, state->dtype, act, a->dtype == GDNR_DTYPE_F32, stream));
+}
+
+int gdnr_qkv_norm_rope_append(const gdnr_tensor* q, const gdnr_tensor* k, const gdnr_tensor* v, const gdnr_tensor* q_weight,
+                              const gdnr_tensor* k_weight, const gdnr_tensor* cos_sin, const gdnr_tensor* positions,
+                              const gdnr_tensor* k_cache, const gdnr_tensor* v_cache, const gdnr_tensor* slot_mapping,
+                              const gdnr_tensor* q_out, int32_t interleaved, float eps, void* stream) {
+  g_last_error.clear();
+  if (!(eps >= 0.0f && eps - eps == 0.0f)) return fail(GDNR_ERR_INVALID_ARGUMENT, "eps: %g is not a finite number >= 0", (double)eps);
+  GDNR_TRY(check_desc(q, "q", 3));
+  const int act = q->dtype;
+  if (!is_act16(act)) return fail(GDNR_ERR_UNSUPPORTED, "q: dtype %s (bf16 and f16 are built)", dtype_name(act));
+  const int64_t T = q->shape[0], HQ = q->shape[1], D = q->shape[2];
+  GDNR_TRY(check_head_dim(D));
+  GDNR_TRY(check_desc(k, "k", 3));
+  const int64_t HKV = k->shape[1];
+  GDNR_TRY(check_act_tensor(q, "q", 3, {T, HQ, D}, act, 16));
+  GDNR_TRY(check_act_tensor(k, "k", 3, {T, HKV, D}, act, 16));
+  GDNR_TRY(check_act_tensor(v, "v", 3, {T, HKV, D}, act, 16));
+  GDNR_TRY(check_act_tensor(q_out, "q_out", 3, {T, HQ, D}, act, 16));
+  for (const auto& w : {std::pair<const gdnr_tensor*, const char*>{q_weight, "q_weight"}, {k_weight, "k_weight"}}) {
+    if (!w.first) continue;
+    GDNR_TRY(check_desc(w.first, w.second, 1));
+    GDNR_TRY(check_dtype(w.first, w.second, {GDNR_DTYPE_F32}));
+    GDNR_TRY(check_shape(w.first, w.second, {D}));
+    GDNR_TRY(check_inner_unit(w.first, w.second));
+  }
+  GDNR_TRY(check_desc(cos_sin, "cos_sin", 2));
+  GDNR_TRY(check_dtype(cos_sin, "cos_sin", {GDNR_DTYPE_F32}));
+  GDNR_TRY(check_inner_unit(cos_sin, "cos_sin"));
+  const int64_t P = cos_sin->shape[0], R = cos_sin->shape[1];
+  if (R < 16 || R % 16 || R > D)
+    return fail(GDNR_ERR_INVALID_ARGUMENT, "cos_sin: rotary width %lld is not a multiple of 16 up to the head dim %lld",
+                (long long)R, (long long)D);
+  if (P < 1 || P > INT32_MAX) return fail(GDNR_ERR_INVALID_ARGUMENT, "cos_sin: %lld positions", (long long)P);
+  GDNR_TRY(check_index_vec(positions, "positions", T, false));
+  GDNR_TRY(check_index_vec(slot_mapping, "slot_mapping", T, false));
+  GDNR_TRY(check_cache(k_cache, "k_cache", act, HKV, D));
+  GDNR_TRY(check_cache(v_cache, "v_cache", act, HKV, D));
+  GDNR_TRY(check_shape(v_cache, "v_cache", {k_cache->shape[0], k_cache->shape[1]}));
+  GDNR_TRY(check_tokens(T, 0));
+  if (HQ + 2 * HKV > 4096) return fail(GDNR_ERR_UNSUPPORTED, "%lld heads exceed 4096", (long long)(HQ + 2 * HKV));
+  if (T * (HQ + HKV) == 0) return GDNR_OK;
+  gdnr::AppendArgs r = {};
+  r.q = q->data, r.q_t = q->strides[0], r.q_h = q->strides[1];
+  r.k = k->data, r.k_t = k->strides[0], r.k_h = k->strides[1];
+  r.v = v->data, r.v_t = v->strides[0], r.v_h = v->strides[1];
+  r.q_weight = q_weight ? (const float*)q_weight->data : nullptr;
+  r.k_weight = k_weight ? (const float*)k_weight->data : nullptr;
+  r.table = (const float*)cos_sin->data, r.tb_p = cos_sin->strides[0];
+  r.position = (const int32_t*)positions->data, r.po_s = positions->strides[0];
+  r.slot = (const int32_t*)slot_mapping->data, r.sl_s = slot_mapping->strides[0];
+  r.k_cache = k_cache->data, r.kc_p = k_cache->strides[0], r.kc_t = k_cache->strides[1], r.kc_h = k_cache->strides[2];
+  r.v_cache = v_cache->data, r.vc_p = v_cache->strides[0], r.vc_t = v_cache->strides[1], r.vc_h = v_cache->strides[2];
+  r.q_out = q_out->data, r.qo_t = q_out->strides[0], r.qo_h = q_out->strides[1];
+  r.T = (int32_t)T, r.HQ = (int32_t)HQ, r.HKV = (int32_t)HKV, r.D = (int32_t)D, r.rotary = (int32_t)R;
+  r.positions = (int32_t)P, r.page = (int32_t)k_cache->shape[1], r.interleaved = interleaved != 0;
+  r.slots = k_cache->shape[0] * k_cache->shape[1], r.eps = eps;
+  return hip_status(gdnr::launch_append(r, act, stream));
+}
+
+int64_t gdnr_paged_attention_workspace(int64_t tokens, int64_t sequences, int32_t heads, int32_t kv_heads,
+                                       int32_t head_dim, int64_t max_context) {
+  g_last_error.clear();
+  if (tokens < 0 || sequences < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || max_context < 0 || max_context > INT32_MAX) {
+    fail(GDNR_ERR_INVALID_ARGUMENT, "tokens, sequences and max_context must not be negative, heads a multiple of kv_heads");
+    return -1;
+  }
+  int32_t piece, pieces;
+  attention_pieces(tokens, sequences, heads, kv_heads, max_context, &piece, &pieces);
+  return attention_workspace(tokens, heads, head_dim, pieces);
+}
+
+int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const gdnr_tensor* v_cache,
+                         const gdnr_tensor* block_table, const gdnr_tensor* cu_seqlens, const gdnr_tensor* context_lens,
+                         const gdnr_tensor* out, const gdnr_tensor* workspace, int32_t max_context, float scale,
+                         void* stream) {
+  g_last_error.clear();
+  if (!(scale - scale == 0.0f)) return fail(GDNR_ERR_INVALID_ARGUMENT, "scale: %g is not finite", (double)scale);
+  GDNR_TRY(check_desc(q, "q", 3));
+  const int act = q->dtype;
+  if (!is_act16(act)) return fail(GDNR_ERR_UNSUPPORTED, "q: dtype %s (bf16 and f16 are built)", dtype_name(act));
+  const int64_t T = q->shape[0], HQ = q->shape[1], D = q->shape[2];
+  GDNR_TRY(check_head_dim(D));
+  GDNR_TRY(check_desc(k_cache, "k_cache", 4));
+  const int64_t HKV = k_cache->shape[2];
+  if (HKV < 1 || HQ < 1 || HQ % HKV)
+    return fail(GDNR_ERR_INVALID_ARGUMENT, "%lld key heads do not divide %lld query heads", (long long)HKV, (long long)HQ);
+  GDNR_TRY(check_act_tensor(q, "q", 3, {T, HQ, D}, act, 16));
+  GDNR_TRY(check_act_tensor(out, "out", 3, {T, HQ, D}, act, 16));
+  GDNR_TRY(check_cache(k_cache, "k_cache", act, HKV, D));
+  GDNR_TRY(check_cache(v_cache, "v_cache", act, HKV, D));
+  GDNR_TRY(check_shape(v_cache, "v_cache", {k_cache->shape[0], k_cache->shape[1]}));
+  int64_t N;
+  GDNR_TRY(check_starts(cu_seqlens, &N));
+  GDNR_TRY(check_index_vec(context_lens, "context_lens", N, false));
+  GDNR_TRY(check_desc(block_table, "block_table", 2));
+  GDNR_TRY(check_dtype(block_table, "block_table", {GDNR_DTYPE_I32}));
+  GDNR_TRY(check_shape(block_table, "block_table", {N}));
+  GDNR_TRY(check_inner_unit(block_table, "block_table"));
+  const int64_t pages = k_cache->shape[0], page = k_cache->shape[1], held = block_table->shape[1] * page;
+  if (max_context < 0 || max_context > held)
+    return fail(GDNR_ERR_INVALID_ARGUMENT, "max_context=%d outside [0, %lld] (block_table's width by the page)", max_context,
+                (long long)held);
+  if (max_context > 0 && pages == 0 && N > 0) return fail(GDNR_ERR_INVALID_ARGUMENT, "k_cache holds no page");
+  GDNR_TRY(check_tokens(T, N));
+  if (HQ > 4096) return fail(GDNR_ERR_UNSUPPORTED, "%lld heads exceed 4096", (long long)HQ);
+  if (T * N == 0) return GDNR_OK;
+  gdnr::AttentionArgs r = {};
+  attention_pieces(T, N, HQ, HKV, max_context, &r.piece, &r.pieces);
+  if (r.pieces > 65535) return fail(GDNR_ERR_UNSUPPORTED, "%d pieces of the context exceed 65535", r.pieces);
+  GDNR_TRY(check_workspace(workspace, attention_workspace(T, HQ, D, r.pieces)));
+  r.q = q->data, r.q_t = q->strides[0], r.q_h = q->strides[1];
+  r.k_cache = k_cache->data, r.kc_p = k_cache->strides[0], r.kc_t = k_cache->strides[1], r.kc_h = k_cache->strides[2];
+  r.v_cache = v_cache->data, r.vc_p = v_cache->strides[0], r.vc_t = v_cache->strides[1], r.vc_h = v_cache->strides[2];
+  r.table = (const int32_t*)block_table->data, r.tb_n = block_table->strides[0], r.table_width = (int32_t)block_table->shape[1];
+  r.cu = (const int32_t*)cu_seqlens->data, r.cu_s = cu_seqlens->strides[0];
+  r.context = (const int32_t*)context_lens->data, r.cx_s = context_lens->strides[0];
+  r.out = out->data, r.o_t = out->strides[0], r.o_h = out->strides[1];
+  if (r.pieces > 1) {
+    r.part = (float*)workspace->data;
+    r.part_ml = r.part + (int64_t)r.pieces * T * HQ * D;
+  }
+  r.T = (int32_t)T, r.N = (int32_t)N, r.HQ = (int32_t)HQ, r.HKV = (int32_t)HKV, r.G = (int32_t)(HQ / HKV), r.D = (int32_t)D;
+  r.page = (int32_t)page, r.n_pages = (int32_t)pages, r.max_context = max_context;
+  r.scale_log2 = scale * 1.4426950408889634f;
+  return hip_status(gdnr::launch_attention(r, act, stream));
 }
 
 }  // extern "C"

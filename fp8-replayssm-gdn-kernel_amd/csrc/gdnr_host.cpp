@@ -62,7 +62,8 @@ constexpr Signature signature() {
 constexpr Signature kSignatures[] = {
     signature<1, 1>(),  signature<3, 0>(),  signature<3, 2>(),  signature<4, 0>(),     signature<4, 2>(),
     signature<7, 0>(),  signature<9, 3>(),  signature<10, 1>(), signature<11, 1>(),    signature<11, 3>(),
-    signature<16, 1>(), signature<17, 1>(), signature<8, 0, 1>(),
+    signature<16, 1>(), signature<17, 1>(), signature<8, 0, 1>(), signature<8, 1, 1>(), signature<11, 0, 1>(),
+    signature<11, 1, 1>(),
 };
 
 struct Entry {

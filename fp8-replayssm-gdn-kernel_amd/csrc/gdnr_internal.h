@@ -165,6 +165,60 @@ struct RmwArgs {
   const int32_t* slot; int64_t sl_s; int32_t n_slots, H;
 };
 
+// Gated delta rule over packed sequences (gdnr_prefill.hip): sequence n owns
+// the token rows [cu[n], cu[n + 1]) (clamped to [0, T]) and the state of slot
+// slot[n]. The state strides are in state elements, the others in activation
+// elements.
+struct PrefillArgs {
+  const void* mixed; int64_t mx_t;
+  const void* a; int64_t a_t, a_h;
+  const void* bgate; int64_t bg_t, bg_h;
+  const float* a_log; int64_t al_s;
+  const float* dt_bias; int64_t db_s;
+  void* state; int64_t st_s, st_h, st_v;
+  const int32_t* slot; int64_t sl_s; int32_t n_slots;
+  const int32_t* cu; int64_t cu_s;
+  const uint8_t* started; int64_t sd_s;  // nullptr: every sequence continues from its slot's state
+  void* out; int64_t o_t, o_h;
+  int32_t T, N, H, HV, V, G;
+  float out_scale;
+};
+
+// Head norms, position rotation and append to a paged cache
+// (gdnr_append.hip). Strides in elements of the tensor they index.
+struct AppendArgs {
+  const void* q; int64_t q_t, q_h;
+  const void* k; int64_t k_t, k_h;
+  const void* v; int64_t v_t, v_h;
+  const float* q_weight; const float* k_weight;  // nullptr: no norm
+  const float* table; int64_t tb_p;              // [positions, rotary]: cosines, then sines
+  const int32_t* position; int64_t po_s;
+  const int32_t* slot; int64_t sl_s;
+  void* k_cache; int64_t kc_p, kc_t, kc_h;
+  void* v_cache; int64_t vc_p, vc_t, vc_h;
+  void* q_out; int64_t qo_t, qo_h;
+  int32_t T, HQ, HKV, D, rotary, positions, page, interleaved, splits;
+  int64_t slots;                                 // pages * page
+  float eps;
+};
+
+// Attention of new tokens over a paged cache (gdnr_attention.hip). Strides
+// in elements of the tensor they index.
+struct AttentionArgs {
+  const void* q; int64_t q_t, q_h;
+  const void* k_cache; int64_t kc_p, kc_t, kc_h;
+  const void* v_cache; int64_t vc_p, vc_t, vc_h;
+  const int32_t* table; int64_t tb_n; int32_t table_width;
+  const int32_t* cu; int64_t cu_s;
+  const int32_t* context; int64_t cx_s;
+  void* out; int64_t o_t, o_h;
+  float* part;       // [pieces, T, HQ, D] sums of p v, unnormalised
+  float* part_ml;    // [pieces, T, HQ, 2] running maximum and sum
+  int32_t T, N, HQ, HKV, G, D, page, n_pages, max_context;
+  int32_t piece, pieces;  // keys a workgroup walks, and the most pieces a context has
+  float scale_log2;       // scale * log2(e)
+};
+
 // Launch modes of the replay kernel.
 enum ReplayMode : int { kModeReplay = 0, kModeApply = 1, kModeFused = 2 };
 
@@ -206,6 +260,9 @@ constexpr int64_t kSplitScratchBytes = 3 << 20;
 uint8_t* split_scratch();
 int launch_rmw_step(const RmwArgs& a, int state_dt, int act_dt, void* stream);
 int launch_rmw_packed(const RmwArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream);
+int launch_prefill(const PrefillArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream);
+int launch_append(const AppendArgs& a, int act_dt, void* stream);
+int launch_attention(const AttentionArgs& a, int act_dt, void* stream);
 int launch_format_quantize(const FormatArgs& a, void* stream);
 int launch_format_dequantize(const FormatArgs& a, void* stream);
 // coalesced stream over bytes (a multiple of 16) at buf: read only, or read

@@ -75,6 +75,9 @@ ENTRY_POINTS = {
     "gdnr_quantize_checkpoint": (4, 2),
     "gdnr_dequantize_checkpoint": (3, 2),
     "gdnr_stream_probe": (1, 1),
+    "gdnr_prefill": (11, 0, 1),
+    "gdnr_qkv_norm_rope_append": (11, 1, 1),
+    "gdnr_paged_attention": (8, 1, 1),
 }
 
 # position of each entry point in the extension's table
@@ -104,6 +107,10 @@ def load_library(path: Path | None = None) -> ctypes.CDLL:
     lib.gdnr_set_wait_polls.argtypes = [ctypes.c_uint32]
     lib.gdnr_decode_plan.restype = ctypes.c_int
     lib.gdnr_decode_plan.argtypes = [ctypes.c_int32] * 6 + [ctypes.POINTER(ctypes.c_int32)]
+    lib.gdnr_prefill_workspace.restype = ctypes.c_int64
+    lib.gdnr_prefill_workspace.argtypes = [ctypes.c_int64] * 2 + [ctypes.c_int32] * 5
+    lib.gdnr_paged_attention_workspace.restype = ctypes.c_int64
+    lib.gdnr_paged_attention_workspace.argtypes = [ctypes.c_int64] * 2 + [ctypes.c_int32] * 3 + [ctypes.c_int64]
     for name, (n_tensors, n_ints, *n_floats) in ENTRY_POINTS.items():
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
@@ -185,3 +192,23 @@ def decode_plan(batch: int, heads: int, value_heads: int, value_dim: int, ring_l
         raise GdnrError(status, lib.gdnr_last_error().decode())
     return {"rows_per_wave": plan[0], "waves_per_head": plan[1], "heads_per_unit": plan[2], "units": plan[3],
             "lds_bytes": plan[4]}
+
+
+def _workspace_bytes(count: int) -> int:
+    if count < 0:
+        raise GdnrError(1, load_library().gdnr_last_error().decode())
+    return count
+
+
+def prefill_workspace(tokens: int, sequences: int, heads: int, value_heads: int, value_dim: int, act: torch.dtype,
+                      state: torch.dtype) -> int:
+    """Bytes of workspace of a gdnr_prefill call (gdnr_prefill_workspace)."""
+    return _workspace_bytes(load_library().gdnr_prefill_workspace(tokens, sequences, heads, value_heads, value_dim,
+                                                                  DTYPE_CODES.get(act, -1), DTYPE_CODES.get(state, -1)))
+
+
+def paged_attention_workspace(tokens: int, sequences: int, heads: int, kv_heads: int, head_dim: int,
+                              max_context: int) -> int:
+    """Bytes of workspace of a gdnr_paged_attention call (gdnr_paged_attention_workspace)."""
+    return _workspace_bytes(load_library().gdnr_paged_attention_workspace(tokens, sequences, heads, kv_heads, head_dim,
+                                                                          max_context))

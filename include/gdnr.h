@@ -355,6 +355,88 @@ int gdnr_dequantize_checkpoint(const gdnr_tensor* payload, const gdnr_tensor* sc
                                const gdnr_tensor* state, int32_t granularity, int32_t tile_size,
                                void* stream);
 
+/*
+ * The gated delta rule over packed sequences of any length (a prompt, a chunk
+ * of one, a few drafted tokens), in the contract of gdnr_bf16_step_packed:
+ * sequence n owns the rows [cu_seqlens[n], cu_seqlens[n + 1]) of mixed_qkv, a,
+ * b and out and the state of slot state_indices[n] (slot 0 the null slot;
+ * out of range -> 0), which its last token's state replaces; per token
+ *   S <- e^g S;  S <- S + beta (v - S k) k^T;  o = scale S q.
+ * has_initial_state (optional, may be NULL: all of them) [N] bool|u8: a
+ * sequence whose entry is 0 starts from a zero state, its slot's contents
+ * unread (one of no tokens leaves zeros there).
+ * Shapes: mixed_qkv [T, 2*H*K + HV*V]; a, b [T,HV] (f32 or the mixed_qkv
+ * dtype); a_log, dt_bias [HV] f32; state [S,HV,V,K] bf16|f16|f32;
+ * state_indices [N] i32; cu_seqlens [N + 1] i32, not decreasing (clamped to
+ * [0, T] on the device); out [T,HV,V] in the mixed_qkv dtype (bf16|f16|f32),
+ * rows outside every sequence unwritten; scale finite. Rows are 16-byte
+ * aligned. K == 128, V % 32 == 0, HV % H == 0, T <= 2^23, N <= 65535. A
+ * non-null slot may appear once.
+ * workspace: u8, gdnr_prefill_workspace bytes (may be NULL where that is 0);
+ * free for other use once the call's kernels have run.
+ * No counterpart in the reference's kernels: its recurrence is run_kernel,
+ * prototype/gdn_replay_fp8_reference.py:137-163; the contract is
+ * findings.md:35-45.
+ */
+int gdnr_prefill(const gdnr_tensor* mixed_qkv, const gdnr_tensor* a, const gdnr_tensor* b,
+                 const gdnr_tensor* a_log, const gdnr_tensor* dt_bias, const gdnr_tensor* state,
+                 const gdnr_tensor* state_indices, const gdnr_tensor* cu_seqlens,
+                 const gdnr_tensor* has_initial_state, const gdnr_tensor* out,
+                 const gdnr_tensor* workspace, float scale, void* stream);
+
+/* Bytes of workspace of a gdnr_prefill call (-1: invalid arguments). Host-only. */
+int64_t gdnr_prefill_workspace(int64_t tokens, int64_t sequences, int32_t heads, int32_t value_heads,
+                               int32_t value_dim, int32_t act_dtype, int32_t state_dtype);
+
+/*
+ * The entry of a full-attention layer in one pass: per head of q and k
+ * x <- w x / sqrt(mean x^2 + eps) (q_weight, k_weight [D] f32, either may be
+ * NULL: no norm), then the rotation of the first R elements by the row
+ * positions[t] (clamped to the table) of cos_sin [P, R] f32 (R/2 cosines, then
+ * R/2 sines): pairs (i, i + R/2), or (2i, 2i + 1) with interleaved != 0; q is
+ * written to q_out, k and v (unchanged) to slot slot_mapping[t] (page *
+ * page_size + offset; outside the cache: nothing is appended) of k_cache and
+ * v_cache. f32 arithmetic, rounded once.
+ * Shapes: q, q_out [T,HQ,D]; k, v [T,HKV,D]; k_cache, v_cache
+ * [pages, page_size, HKV, D]; positions, slot_mapping [T] i32. One dtype,
+ * bf16|f16; D 64, 128 or 256; R a multiple of 16 up to D; 16-byte aligned
+ * rows of any outer strides; two tokens must not share a slot.
+ * No counterpart in the reference (its models' attention layers are vLLM's).
+ */
+int gdnr_qkv_norm_rope_append(const gdnr_tensor* q, const gdnr_tensor* k, const gdnr_tensor* v,
+                              const gdnr_tensor* q_weight, const gdnr_tensor* k_weight,
+                              const gdnr_tensor* cos_sin, const gdnr_tensor* positions,
+                              const gdnr_tensor* k_cache, const gdnr_tensor* v_cache,
+                              const gdnr_tensor* slot_mapping, const gdnr_tensor* q_out,
+                              int32_t interleaved, float eps, void* stream);
+
+/*
+ * Causal attention of new tokens over a paged cache: sequence n owns the rows
+ * [cu_seqlens[n], cu_seqlens[n + 1]) of q and out, and a context of
+ * context_lens[n] keys that ends with its new tokens' (already in the cache);
+ * key i sits at offset i % page_size of page block_table[n, i / page_size].
+ * Token j of L sees the keys i <= context - L + j; a token that sees none
+ * gives 0. out = softmax(scale q k^T) v per query head, head h reading key
+ * head h / (HQ / HKV).
+ * Shapes: q, out [T,HQ,D]; k_cache, v_cache [pages, page_size, HKV, D];
+ * block_table [N, width] i32; cu_seqlens [N + 1], context_lens [N] i32. One
+ * dtype, bf16|f16; D 64, 128 or 256; HQ % HKV == 0; any page size; 16-byte
+ * aligned rows of any outer strides. max_context (at most width * page_size)
+ * bounds context_lens: a longer one is cut to it.
+ * workspace: u8, gdnr_paged_attention_workspace bytes (may be NULL where that
+ * is 0); free for other use once the call's kernels have run.
+ * No counterpart in the reference (its models' attention layers are vLLM's).
+ */
+int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const gdnr_tensor* v_cache,
+                         const gdnr_tensor* block_table, const gdnr_tensor* cu_seqlens,
+                         const gdnr_tensor* context_lens, const gdnr_tensor* out,
+                         const gdnr_tensor* workspace, int32_t max_context, float scale, void* stream);
+
+/* Bytes of workspace of a gdnr_paged_attention call (-1: invalid arguments).
+ * Host-only (it reads the current device's compute-unit count). */
+int64_t gdnr_paged_attention_workspace(int64_t tokens, int64_t sequences, int32_t heads, int32_t kv_heads,
+                                       int32_t head_dim, int64_t max_context);
+
 #ifdef __cplusplus
 }
 #endif
