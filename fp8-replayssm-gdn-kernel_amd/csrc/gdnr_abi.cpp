@@ -1370,13 +1370,13 @@ int64_t attention_workspace(int64_t T, int64_t HQ, int64_t D, int32_t pieces) {
 
 int64_t gdnr_prefill_workspace(int64_t tokens, int64_t sequences, int32_t heads, int32_t value_heads, int32_t value_dim,
                                int32_t act_dtype, int32_t state_dtype) {
-  (void)heads, (void)value_heads, (void)value_dim, (void)act_dtype, (void)state_dtype;
+  (void)value_dim;
   g_last_error.clear();
-  if (tokens < 0 || sequences < 0) {
-    fail(GDNR_ERR_INVALID_ARGUMENT, "tokens and sequences must not be negative");
+  if (tokens < 0 || sequences < 0 || heads < 0 || value_heads < 0) {
+    fail(GDNR_ERR_INVALID_ARGUMENT, "tokens, sequences and heads must not be negative");
     return -1;
   }
-  return 0;
+  return gdnr::prefill_work_bytes(tokens, sequences, heads, value_heads, act_dtype, state_dtype);
 }
 
 int gdnr_prefill(const gdnr_tensor* mixed_qkv, const gdnr_tensor* a, const gdnr_tensor* b, const gdnr_tensor* a_log,
@@ -1443,6 +1443,7 @@ int gdnr_prefill(const gdnr_tensor* mixed_qkv, const gdnr_tensor* a, const gdnr_
   r.out = out->data, r.o_t = out->strides[0], r.o_h = out->strides[1];
   r.T = (int32_t)T, r.N = (int32_t)N, r.H = (int32_t)H, r.HV = (int32_t)HV, r.V = (int32_t)V, r.G = (int32_t)(HV / H);
   r.out_scale = scale;
+  r.work = workspace ? (uint8_t*)workspace->data : nullptr;
   return hip_status(gdnr::launch_prefill(r, state->dtype, act, a->dtype == GDNR_DTYPE_F32, stream));
 }
 

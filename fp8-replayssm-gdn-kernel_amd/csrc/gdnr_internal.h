@@ -182,6 +182,7 @@ struct PrefillArgs {
   void* out; int64_t o_t, o_h;
   int32_t T, N, H, HV, V, G;
   float out_scale;
+  uint8_t* work;  // chunked form: what prefill_work_bytes counts
 };
 
 // Head norms, position rotation and append to a paged cache
@@ -260,6 +261,8 @@ constexpr int64_t kSplitScratchBytes = 3 << 20;
 uint8_t* split_scratch();
 int launch_rmw_step(const RmwArgs& a, int state_dt, int act_dt, void* stream);
 int launch_rmw_packed(const RmwArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream);
+// Bytes of workspace of a gdn prefill (0: the token-by-token form runs)
+int64_t prefill_work_bytes(int64_t T, int64_t N, int32_t H, int32_t HV, int act_dt, int state_dt);
 int launch_prefill(const PrefillArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream);
 int launch_append(const AppendArgs& a, int act_dt, void* stream);
 int launch_attention(const AttentionArgs& a, int act_dt, void* stream);

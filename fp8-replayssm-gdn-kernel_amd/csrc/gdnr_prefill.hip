@@ -161,6 +161,636 @@ __global__ __launch_bounds__(256) void recurrent_kernel(const PrefillArgs a) {
     for (int e = 0; e < 8; e += 2) St::st2(sp + r * srow + e * St::kBytes, S[r][e], S[r][e + 1]);
 }
 
+// ---------------------------------------------------------------- chunked
+// C tokens at once. With G_t = sum of the log decays up to t in the chunk and
+// S0 the state before it,
+//   (I + M) U = beta (V - e^G (K S0^T)),   M_ti = beta_t e^(G_t - G_i) k_t.k_i  (i < t)
+//   O  = scale (e^G (Q S0^T) + A U),       A_ti = e^(G_t - G_i) q_t.k_i         (i <= t)
+//   S1 = e^(G_C) S0 + sum_t e^(G_C - G_t) u_t k_t^T,
+// (U's rows are the corrections beta (v - S k) of the recurrence, unrolled).
+// T = (I + M)^-1 and A depend on the chunk alone: chunk_prep_kernel forms them
+// for every chunk at once, with the unit keys and queries. chunk_scan_kernel
+// then walks a sequence's chunks with matrix products.
+//
+// Numbers: the products run on f16 operands with f32 sums. Unit keys and
+// queries, A and T (|T| <= 1: products of contractions) are safe in f16; V,
+// S0, R and U get a power of two per V-row and chunk, from the largest of the
+// row's v and state, that puts their bound at 2^15 (V-rows do not mix, so each
+// keeps its own precision whatever its neighbours hold). An f16 operand costs
+// 2^-12 of itself, an eighth of what storing bf16 does: bf16 outputs and states
+// are bound by their own rounding. Where a result keeps more than bf16 (f16
+// or f32 activations or state), SPLIT carries every operand as a sum of two
+// f16 values and each product as three, good to some 2^-22. The state between
+// chunks, sums and decays are f32 (the sums of log decays f64, so that
+// differences of long sums stay exact).
+//
+// A token whose key or gates are not finite, and a V-row whose v or state is
+// not, would reach earlier tokens through products with 0: both are computed
+// as zeros and everything from their token on is written as NaN.
+constexpr int C = 64;                   // tokens of a chunk
+constexpr int kTri = 6;                 // 16 x 32 operand tiles of a lower triangle of 64
+constexpr float kFix = 1024.f;          // SPLIT: factor of unit operands, keeps their low halves normal
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2v_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+
+__device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const f32x2v_t v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t w) {
+  const f16x2_t h = __builtin_bit_cast(f16x2_t, w);
+  return make_float2((float)h[0], (float)h[1]);
+}
+
+// 8 values as an MFMA operand: f16, or f16 plus the f16 of what that leaves
+template <bool SPLIT>
+struct Operand {
+  u32x4_t hi, lo;
+};
+template <bool SPLIT>
+__device__ __forceinline__ Operand<SPLIT> operand(f32x4_t a, f32x4_t b) {
+  Operand<SPLIT> o;
+  const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o.hi[i] = pack_f16(x[2 * i], x[2 * i + 1]);
+    if constexpr (SPLIT) {
+      const float2 h = unpack_f16(o.hi[i]);
+      o.lo[i] = pack_f16(x[2 * i] - h.x, x[2 * i + 1] - h.y);
+    }
+  }
+  return o;
+}
+template <bool SPLIT>
+__device__ __forceinline__ f32x4_t product(const Operand<SPLIT>& a, const Operand<SPLIT>& b, f32x4_t c) {
+  if constexpr (SPLIT) {
+    c = mfma(a.lo, b.hi, c);
+    c = mfma(a.hi, b.lo, c);
+  }
+  return mfma(a.hi, b.hi, c);
+}
+
+// Workspace: per chunk slot and key head the unit keys and queries [C][K] f16
+// (SPLIT: high, then low); per slot and value head the operand tiles of T - I
+// and A (64 lanes x 16 bytes each; SPLIT: high, then low) and the tokens'
+// {beta}[C], {e^G}[C], {e^(G_C - G)}[C], first bad token (as an int), pad[3].
+// Sequence n's chunks take the slots from cu[n] / C + n on.
+constexpr int kScalars = 3 * C + 4;
+__host__ __device__ constexpr int64_t unit_bytes(bool split) { return 2 * C * K * 2 * (split ? 2 : 1); }
+__host__ __device__ constexpr int64_t tile_bytes(bool split) { return 2 * kTri * 1024 * (split ? 2 : 1); }
+__host__ __device__ constexpr int64_t head_bytes(bool split) { return tile_bytes(split) + kScalars * 4; }
+
+struct Work {
+  uint8_t* unit;  // [slots][H]
+  uint8_t* head;  // [slots][HV]
+};
+__host__ __device__ inline Work work_of(const PrefillArgs& a, bool split) {
+  const int64_t slots = a.T / C + a.N;
+  return {a.work, a.work + slots * a.H * unit_bytes(split)};
+}
+
+// chunks whose operands the scan keeps in LDS
+__host__ __device__ constexpr int scan_buffers(bool split) { return split ? 1 : 2; }
+
+// index of the tile (16 rows of t, 32 columns of i) in a lower triangle
+__host__ __device__ constexpr int tri(int tt, int ts) { return tt < 2 ? tt : 2 * (tt - 1) + ts; }
+
+__device__ __forceinline__ float exp_diff(double d) {
+  const float h = (float)d;
+  const float e = expf(h);
+  return fmaf(e, (float)(d - (double)h), e);
+}
+
+// One chunk of one key head: 4 waves. The Gram products are formed transposed
+// (rows i on a lane's registers, columns t on lanes), which is the order that
+// the scan's operands take them in.
+template <class Act, bool GATE_F32, bool SPLIT>
+__global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
+  using Gate = typename std::conditional<GATE_F32, ActF32, Act>::type;
+  constexpr int ES = Act::kBytes, RS = 2 * K + 16, P = SPLIT ? 2 : 1;  // LDS row of a key or query, halves
+  constexpr int kUnits = 2 * P * C * RS, MS = 68 * 4, kM = C * MS;      // [i][t] f32 of M, per head
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kUnits > 2 * kM ? kUnits : 2 * kM];
+  __shared__ double Gs[2][C];
+  __shared__ float betas[2][C];
+  __shared__ int bad_key;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int slot = blockIdx.x, h = blockIdx.y;
+
+  // the slot's sequence and first row
+  int n = -1;
+  for (int n0 = 0; n0 < a.N; n0 += 64) {
+    bool below = false;
+    if (n0 + lane < a.N) below = min(max(a.cu[(n0 + lane) * a.cu_s], 0), a.T) / C + n0 + lane <= slot;
+    n += __popcll(__ballot(below));
+  }
+  if (n < 0) return;
+  int begin, end;
+  sequence_rows(a, n, begin, end);
+  const int row0 = begin + (slot - begin / C - n) * C, len = min(end - row0, C);
+  if (len <= 0) return;
+  const Work w = work_of(a, SPLIT);
+  if (threadIdx.x == 0) bad_key = C;
+  __syncthreads();
+
+  // unit keys and queries, 16 lanes a row
+  uint8_t* unit = w.unit + ((int64_t)slot * a.H + h) * unit_bytes(SPLIT);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool is_q = i >= 4;
+    const int t = 16 * (i & 3) + 4 * wave + grp;
+    float x[8], ss = 0.f;
+    Raw<Act, 8> r;
+    if (t < len) r.load((const uint8_t*)a.mixed + ((int64_t)(row0 + t) * a.mx_t + (is_q ? h : a.H + h) * K + 8 * col) * ES);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = t < len ? r[e] : 0.f, ss = fmaf(x[e], x[e], ss);
+    ss = sum16(ss);
+    float f = 1.f / sqrtf(ss + 1e-6f);
+    if (!is_q && !(ss < __builtin_inff())) {
+      if (col == 0) atomicMin(&bad_key, t);
+      f = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    }
+    if constexpr (SPLIT) f *= kFix;
+    const Operand<SPLIT> o = operand<SPLIT>(f32x4_t{x[0] * f, x[1] * f, x[2] * f, x[3] * f}, f32x4_t{x[4] * f, x[5] * f, x[6] * f, x[7] * f});
+    const int plane = (is_q ? P : 0);
+    *(u32x4_t*)(lds + (plane * C + t) * RS + 16 * col) = o.hi;
+    *(u32x4_t*)(unit + (plane * C + t) * (2 * K) + 16 * col) = o.hi;
+    if constexpr (SPLIT) {
+      *(u32x4_t*)(lds + ((plane + 1) * C + t) * RS + 16 * col) = o.lo;
+      *(u32x4_t*)(unit + ((plane + 1) * C + t) * (2 * K) + 16 * col) = o.lo;
+    }
+  }
+  __syncthreads();
+
+  // wave w: columns t of tile w, rows i of tiles 0..w
+  f32x4_t kk[4], qk[4];
+  auto fragment = [&](int plane, int tile, int step) {
+    Operand<SPLIT> o;
+    o.hi = *(const u32x4_t*)(lds + (plane * C + 16 * tile + col) * RS + 64 * step + 16 * grp);
+    if constexpr (SPLIT) o.lo = *(const u32x4_t*)(lds + ((plane + 1) * C + 16 * tile + col) * RS + 64 * step + 16 * grp);
+    return o;
+  };
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    kk[c] = f32x4_t{0.f, 0.f, 0.f, 0.f}, qk[c] = kk[c];
+    if (c > wave) continue;
+#pragma unroll
+    for (int s = 0; s < K / 32; ++s) {
+      const Operand<SPLIT> ki = fragment(0, c, s);
+      kk[c] = product<SPLIT>(ki, fragment(0, wave, s), kk[c]);
+      qk[c] = product<SPLIT>(ki, fragment(P, wave, s), qk[c]);
+    }
+    if constexpr (SPLIT) kk[c] *= 1.f / (kFix * kFix), qk[c] *= 1.f / kFix;  // (A keeps one factor)
+  }
+
+  // the group's value heads, two at a time
+  for (int g0 = 0; g0 < a.G; g0 += 2) {
+    const int heads = min(2, a.G - g0);
+    __syncthreads();  // the units (or the last heads' M) are no longer read
+    if (wave < heads) {
+      const int hv = h * a.G + g0 + wave, t = lane;
+      const int64_t at = row0 + t;
+      float g = 0.f, beta = 0.f;
+      bool bad = t >= bad_key;
+      if (t < len) {
+        g = log_decay(Gate::ld(a.a, at * a.a_t + hv * a.a_h) + a.dt_bias[hv * a.db_s], a.a_log[hv * a.al_s]);
+        beta = sigmoid(Gate::ld(a.bgate, at * a.bg_t + hv * a.bg_h));
+        bad |= g != g || beta != beta || g > 3e38f;
+      }
+      const uint64_t bads = __ballot(bad && t < len);
+      const int first = bads ? __ffsll((unsigned long long)bads) - 1 : C;
+      if (t >= first) g = 0.f, beta = 0.f;
+      // (a decay of e^-1e4 is 0 in every format; a sum of such stays exact)
+      double G = fmaxf(g, -1e4f);
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const double up = __shfl_up(G, d);
+        if (lane >= d) G += up;
+      }
+      const double last = __shfl(G, 63);
+      Gs[wave][t] = G;
+      betas[wave][t] = beta;
+      float* sc = (float*)(w.head + ((int64_t)slot * a.HV + hv) * head_bytes(SPLIT) + tile_bytes(SPLIT));
+      sc[t] = beta;
+      sc[C + t] = exp_diff(G);
+      sc[2 * C + t] = exp_diff(last - G);
+      if (t == 0) ((int*)sc)[3 * C] = first;
+    }
+    __syncthreads();
+    for (int e = 0; e < heads; ++e) {
+      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + e) * head_bytes(SPLIT);
+      const int t = 16 * wave + col;
+      const double Gt = Gs[e][t];
+      const float bt = betas[e][t];
+      f32x4_t at[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        at[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (c > wave) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 16 * c + 4 * grp + j;
+          const float decay = i <= t ? exp_diff(Gt - Gs[e][i]) : 0.f;
+          at[c][j] = i <= t ? decay * qk[c][j] : 0.f;
+          *(float*)(lds + e * kM + i * MS + t * 4) = i < t ? bt * decay * kk[c][j] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (2 * s > wave) continue;
+        const Operand<SPLIT> o = operand<SPLIT>(at[2 * s], at[2 * s + 1]);
+        uint8_t* p = tiles + (kTri * P + tri(wave, s)) * 1024 + 16 * lane;
+        *(u32x4_t*)p = o.hi;
+        if constexpr (SPLIT) *(u32x4_t*)(p + kTri * 1024) = o.lo;
+      }
+    }
+    __syncthreads();
+    if (wave < heads) {
+      // row t of T, one lane each: x (I + M) = e_t, from the last column on
+      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + wave) * head_bytes(SPLIT);
+      const uint8_t* m = lds + wave * kM;
+      float x[C];
+#pragma unroll
+      for (int i = C - 1; i >= 0; --i) {
+        float acc[2] = {lane == i ? 1.f : 0.f, 0.f};
+#pragma unroll
+        for (int j0 = (i + 1) & ~3; j0 < C; j0 += 4) {
+          const f32x4_t mj = *(const f32x4_t*)(m + i * MS + j0 * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j0 + j > i) acc[j & 1] = fmaf(-x[j0 + j], mj[j], acc[j & 1]);
+        }
+        x[i] = acc[0] + acc[1];
+      }
+#pragma unroll
+      for (int i = 0; i < C; ++i) x[i] = lane == i ? 0.f : SPLIT ? x[i] * kFix : x[i];  // T - I
+      const int tt = lane >> 4;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (2 * s <= tt) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int i = 32 * s + 4 * g;
+            const Operand<SPLIT> o = operand<SPLIT>(f32x4_t{x[i], x[i + 1], x[i + 2], x[i + 3]},
+                                                    f32x4_t{x[i + 16], x[i + 17], x[i + 18], x[i + 19]});
+            uint8_t* p = tiles + tri(tt, s) * 1024 + 16 * (16 * g + col);
+            *(u32x4_t*)p = o.hi;
+            if constexpr (SPLIT) *(u32x4_t*)(p + kTri * 1024) = o.lo;
+          }
+        }
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+// over the lanes of one column (lane & 15), in each of them
+__device__ __forceinline__ uint32_t column_max(uint32_t x) {
+  x = max(x, (uint32_t)__shfl_xor((int)x, 16));
+  return max(x, (uint32_t)__shfl_xor((int)x, 32));
+}
+
+// A sequence's chunks in order, for 16 NV V-rows of one value head a wave,
+// WAVES waves sharing a chunk's operands in LDS. A wave's V-rows are the
+// columns (lane & 15) of every product, so what one product leaves in
+// registers (rows k or t: 4 grp + j of a 16-row tile) is the next one's
+// operand as it stands: both operands of a product may take its contraction in
+// any order, and the keys', T's and A's fragments are read in that one.
+template <class Act, class St, bool SPLIT, int WAVES, int NV>
+__global__ __launch_bounds__(64 * WAVES) void chunk_scan_kernel(const PrefillArgs a) {
+  constexpr int ES = Act::kBytes, P = SPLIT ? 2 : 1, RS = 2 * K + 32;  // LDS row: 16 rows' 32-byte pieces on distinct banks
+  constexpr int THREADS = 64 * WAVES, kUnitRows = 2 * P * C, kUnits = kUnitRows * RS;
+  constexpr int kHead = (int)head_bytes(SPLIT), kBuf = kUnits + kHead;
+  constexpr int BUFS = scan_buffers(SPLIT);
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  constexpr int COLS = 16 * NV * WAVES;
+  const int blocks = a.V / COLS, hv = blockIdx.x / blocks, n = blockIdx.y;
+  const int v0 = (blockIdx.x - hv * blocks) * COLS + wave * 16 * NV + col * NV;  // this lane's V-rows: v0 .. v0 + NV - 1
+  const int h = hv / a.G;
+  int begin, end;
+  sequence_rows(a, n, begin, end);
+  const bool started = sequence_started(a, n);
+  if (begin == end && started) return;
+  const Work w = work_of(a, SPLIT);
+  const int slot0 = begin / C + n, chunks = (end - begin + C - 1) / C;
+
+  // the state, transposed: tile kt of 16 columns k, rows 4 grp + j
+  uint8_t* sp = (uint8_t*)a.state + ((int64_t)sequence_slot(a, n) * a.st_s + hv * a.st_h + (int64_t)v0 * a.st_v + 4 * grp) * St::kBytes;
+  f32x4_t S[NV][8];  // times sc[nv]
+  float sc[NV], inv[NV];
+#pragma unroll
+  for (int nv = 0; nv < NV; ++nv) {
+    sc[nv] = inv[nv] = 1.f;
+#pragma unroll
+    for (int kt = 0; kt < 8; ++kt) {
+      Raw<St, 4> x;
+      if (started) x.load(sp + (nv * a.st_v + 16 * kt) * St::kBytes);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[nv][kt][j] = started ? x[j] : 0.f;
+    }
+  }
+
+  // a chunk's operands: global -> registers (while the chunk before is
+  // computed) -> LDS
+  constexpr int kPieces = (kUnitRows * 16 + kHead / 16 + THREADS - 1) / THREADS;
+  u32x4_t piece[kPieces];
+  auto fetch = [&](int c) {
+    const uint8_t* unit = w.unit + ((int64_t)(slot0 + c) * a.H + h) * unit_bytes(SPLIT);
+    const uint8_t* head = w.head + ((int64_t)(slot0 + c) * a.HV + hv) * head_bytes(SPLIT);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int x = i * THREADS + (int)threadIdx.x;
+      if (x < kUnitRows * 16) piece[i] = *(const u32x4_t*)(unit + 16 * x);
+      else if (x < kUnitRows * 16 + kHead / 16) piece[i] = *(const u32x4_t*)(head + 16 * (x - kUnitRows * 16));
+    }
+  };
+  auto stage = [&](int c) {
+    uint8_t* b = lds + (c % BUFS) * kBuf;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int x = i * THREADS + (int)threadIdx.x;
+      if (x < kUnitRows * 16) *(u32x4_t*)(b + (x >> 4) * RS + 16 * (x & 15)) = piece[i];
+      else if (x < kUnitRows * 16 + kHead / 16) *(u32x4_t*)(b + kUnits + 16 * (x - kUnitRows * 16)) = piece[i];
+    }
+  };
+  // the chunk's v: rows t of this lane, NV neighbours each
+  float vn[NV][4][4];
+  const uint8_t* vp = (const uint8_t*)a.mixed + (2 * a.H * K + (int64_t)hv * a.V + v0) * ES;
+  auto fetch_v = [&](int c) {
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = c * C + 16 * tt + 4 * grp + j;
+        const bool on = begin + t < end;
+        const uint8_t* p = vp + (int64_t)min(begin + t, end - 1) * a.mx_t * ES;
+        if constexpr (NV == 2) {
+          const float2 x = Act::ld2(p);
+          vn[0][tt][j] = on ? x.x : 0.f, vn[1][tt][j] = on ? x.y : 0.f;
+        } else {
+          const float x = Act::ld(p, 0);
+          vn[0][tt][j] = on ? x : 0.f;
+        }
+      }
+  };
+
+  if (chunks) fetch(0), fetch_v(0), stage(0);
+  for (int c = 0; c < chunks; ++c) {
+    __syncthreads();  // chunk c's operands are in LDS; those of c - 1 are no longer read
+    const uint8_t* b = lds + (c % BUFS) * kBuf;
+    const uint8_t* head = b + kUnits;
+    const float* scal = (const float*)(head + tile_bytes(SPLIT));
+    float v[NV][4][4];
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[nv][i >> 2][i & 3] = vn[nv][i >> 2][i & 3];
+    if (c + 1 < chunks) fetch(c + 1), fetch_v(c + 1);
+    const int bad_token = __builtin_amdgcn_readfirstlane(((const int*)scal)[3 * C]);
+
+    // V-rows with a value that is not finite: zeros here, NaN from its token on
+    uint32_t ms[NV], mv[NV];
+    auto largest = [&](int nv) {
+      uint32_t x = 0, y = 0;
+#pragma unroll
+      for (int kt = 0; kt < 8; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x = max(x, abs_bits(S[nv][kt][j]));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y = max(y, abs_bits(v[nv][i >> 2][i & 3]));
+      ms[nv] = column_max(x), mv[nv] = column_max(y);
+    };
+    int first[NV];
+    bool any_bad = bad_token < C;
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv) {
+      first[nv] = C;
+      largest(nv);
+      any_bad |= __any(ms[nv] >= 0x7F800000u || mv[nv] >= 0x7F800000u);
+    }
+    if (any_bad) {
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) {
+        uint32_t at = ms[nv] >= 0x7F800000u ? 0 : C;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float& x = v[nv][i >> 2][i & 3];
+          if (abs_bits(x) >= 0x7F800000u) at = min(at, (uint32_t)(16 * (i >> 2) + 4 * grp + (i & 3))), x = 0.f;
+        }
+#pragma unroll
+        for (int kt = 0; kt < 8; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (abs_bits(S[nv][kt][j]) >= 0x7F800000u) S[nv][kt][j] = 0.f;
+        first[nv] = min((int)(C - column_max(C - at)), bad_token);
+        largest(nv);
+      }
+    }
+    // each row's power of two: |R| and |U| are at most 64 (|v| + 12 |S|)
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv) {
+      const float bound = fmaxf(__uint_as_float(mv[nv]), 12.f * __uint_as_float(ms[nv]) * inv[nv]);
+      const uint32_t ex = min(max((__float_as_uint(bound) >> 23) + 7, 15u), 254u);
+      const float s_new = __uint_as_float((268u - ex) << 23), ratio = fminf(s_new * inv[nv], 0x1p126f);
+#pragma unroll
+      for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= ratio;
+      sc[nv] = s_new, inv[nv] = __uint_as_float((ex - 14u) << 23);
+    }
+
+    const f32x4_t* beta4 = (const f32x4_t*)scal;
+    const f32x4_t* grow4 = (const f32x4_t*)(scal + C);
+    const f32x4_t* end4 = (const f32x4_t*)(scal + 2 * C);
+    const float total = scal[2 * C - 1];
+    auto rows_of = [&](int plane, int tile, int step) {  // 16 tokens by 32 columns k
+      Operand<SPLIT> o;
+      const uint8_t* p = b + (plane * C + 16 * tile + col) * RS + 64 * step + 8 * grp;
+      const uint2 x = *(const uint2*)p, y = *(const uint2*)(p + 32);
+      o.hi = u32x4_t{x.x, x.y, y.x, y.y};
+      if constexpr (SPLIT) {
+        const uint2 z = *(const uint2*)(p + C * RS), u = *(const uint2*)(p + C * RS + 32);
+        o.lo = u32x4_t{z.x, z.y, u.x, u.y};
+      }
+      return o;
+    };
+    auto turned = [&](int tile, int step) {  // 16 columns k of the keys by 32 tokens
+      Operand<SPLIT> o;
+      const uint8_t* p = b + (32 * step + 4 * grp + (col >> 2)) * RS + 32 * tile + 8 * (col & 3);
+      auto read = [](const uint8_t* q) { return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q)); };
+      const uint2 x = read(p), y = read(p + 16 * RS);
+      o.hi = u32x4_t{x.x, x.y, y.x, y.y};
+      if constexpr (SPLIT) {
+        const uint2 z = read(p + C * RS), u = read(p + (C + 16) * RS);
+        o.lo = u32x4_t{z.x, z.y, u.x, u.y};
+      }
+      return o;
+    };
+    auto triangle = [&](int base, int tt, int ts) {
+      Operand<SPLIT> o;
+      const uint8_t* p = head + (base * P + tri(tt, ts)) * 1024 + 16 * lane;
+      o.hi = *(const u32x4_t*)p;
+      if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + kTri * 1024);
+      return o;
+    };
+    constexpr float kUp = SPLIT ? kFix : 1.f, kDown = 1.f / kUp;
+
+    Operand<SPLIT> bs[NV][4];
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) bs[nv][s] = operand<SPLIT>(S[nv][2 * s], S[nv][2 * s + 1]);
+    // R = beta (v - e^G (K S0^T)), U = R + (T - I) R
+    f32x4_t u[NV][4];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      f32x4_t x[NV];
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) x[nv] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const Operand<SPLIT> k = rows_of(0, tt, s);
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) x[nv] = product<SPLIT>(k, bs[nv][s], x[nv]);
+      }
+      const f32x4_t be = beta4[4 * tt + grp], gr = grow4[4 * tt + grp];
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[nv][tt][j] = be[j] * (v[nv][tt][j] * sc[nv] - gr[j] * kDown * x[nv][j]);
+    }
+    Operand<SPLIT> ub[NV][2], ud[NV][2];
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) ub[nv][s] = operand<SPLIT>(u[nv][2 * s], u[nv][2 * s + 1]);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv)
+        if constexpr (SPLIT) u[nv][tt] *= kUp;
+#pragma unroll
+      for (int s = 0; s <= tt / 2; ++s) {
+        const Operand<SPLIT> m = triangle(0, tt, s);
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) u[nv][tt] = product<SPLIT>(m, ub[nv][s], u[nv][tt]);
+      }
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv)
+        if constexpr (SPLIT) u[nv][tt] *= kDown;
+    }
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        ub[nv][s] = operand<SPLIT>(u[nv][2 * s], u[nv][2 * s + 1]);
+        ud[nv][s] = operand<SPLIT>(u[nv][2 * s] * end4[8 * s + grp], u[nv][2 * s + 1] * end4[8 * s + 4 + grp]);
+      }
+    // the state after the chunk
+#pragma unroll
+    for (int kt = 0; kt < 8; ++kt) {
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) S[nv][kt] *= total * kUp;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const Operand<SPLIT> k = turned(kt, s);
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) S[nv][kt] = product<SPLIT>(k, ud[nv][s], S[nv][kt]);
+      }
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv)
+        if constexpr (SPLIT) S[nv][kt] *= kDown;
+    }
+    // the outputs
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      f32x4_t o[NV];
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) o[nv] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const Operand<SPLIT> q = rows_of(P, tt, s);
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) o[nv] = product<SPLIT>(q, bs[nv][s], o[nv]);
+      }
+      const f32x4_t gr = grow4[4 * tt + grp];
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) o[nv] *= gr;
+#pragma unroll
+      for (int s = 0; s <= tt / 2; ++s) {
+        const Operand<SPLIT> m = triangle(kTri, tt, s);
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) o[nv] = product<SPLIT>(m, ub[nv][s], o[nv]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = 16 * tt + 4 * grp + j;
+        if (c * C + t >= end - begin) continue;
+        uint8_t* p = (uint8_t*)a.out + ((int64_t)(begin + c * C + t) * a.o_t + hv * a.o_h + v0) * ES;
+        float y[NV];
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) {
+          y[nv] = o[nv][j] * kDown * (a.out_scale * inv[nv]);
+          if (any_bad && t >= first[nv]) y[nv] = __builtin_nanf("");
+        }
+        if constexpr (NV == 2) Act::st2(p, y[0], y[1]);
+        else Act::st(p, 0, y[0]);
+      }
+    }
+    if (any_bad) {
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv)
+        if (first[nv] < C)
+#pragma unroll
+          for (int kt = 0; kt < 8; ++kt) S[nv][kt] = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+    }
+    if constexpr (BUFS == 1) __syncthreads();
+    if (c + 1 < chunks) stage(c + 1);
+  }
+#pragma unroll
+  for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+    for (int kt = 0; kt < 8; ++kt)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2)
+        St::st2(sp + (nv * a.st_v + 16 * kt + j) * St::kBytes, S[nv][kt][j] * inv[nv], S[nv][kt][j + 1] * inv[nv]);
+}
+
+// Whether results keep more than bf16 does.
+bool needs_split(int act_dt, int state_dt) { return act_dt != DT_BF16 || state_dt != DT_BF16; }
+
+// The chunked form from an average of 16 tokens a sequence on.
+bool chunked_form(int64_t T, int64_t N) { return T >= 16 * N; }
+
+template <class Act, bool GATE_F32, bool SPLIT>
+int launch_prep(const PrefillArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((chunk_prep_kernel<Act, GATE_F32, SPLIT>), dim3(a.T / C + a.N, a.H), dim3(256), 0, s, a);
+  return (int)hipGetLastError();
+}
+template <class Act, class St, bool SPLIT, int WAVES, int NV>
+int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
+  constexpr int lds = scan_buffers(SPLIT) * (2 * (SPLIT ? 2 : 1) * C * (2 * K + 32) + (int)head_bytes(SPLIT));
+  static_assert(lds <= kMaxStepLds, "the operands fit");
+  const auto kernel = chunk_scan_kernel<Act, St, SPLIT, WAVES, NV>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e != hipSuccess) return (int)e;
+  hipLaunchKernelGGL(kernel, dim3(a.HV * (a.V / (16 * NV * WAVES)), a.N), dim3(64 * WAVES), lds, s, a);
+  return (int)hipGetLastError();
+}
+template <class Act, class St, bool SPLIT>
+int launch_scan(const PrefillArgs& a, hipStream_t s) {
+  return launch_scan_as<Act, St, SPLIT, 2, 1>(a, s);
+}
+
 template <class Act, class St, bool GATE_F32>
 int launch_recurrent(const PrefillArgs& a, hipStream_t s) {
   const int units = a.HV * (a.V / kRecRows);
@@ -170,12 +800,31 @@ int launch_recurrent(const PrefillArgs& a, hipStream_t s) {
 
 template <class Act, bool GATE_F32>
 int launch_state(const PrefillArgs& a, int state_dt, hipStream_t s) {
+  if (chunked_form(a.T, a.N)) {
+    if constexpr (std::is_same<Act, ActBF16>::value) {
+      if (state_dt == DT_BF16) {
+        const int rc = launch_prep<Act, GATE_F32, false>(a, s);
+        return rc ? rc : launch_scan<Act, ActBF16, false>(a, s);
+      }
+    }
+    const int rc = launch_prep<Act, GATE_F32, true>(a, s);
+    if (rc) return rc;
+    if (state_dt == DT_F16) return launch_scan<Act, ActF16, true>(a, s);
+    if (state_dt == DT_F32) return launch_scan<Act, ActF32, true>(a, s);
+    if constexpr (!std::is_same<Act, ActBF16>::value) return launch_scan<Act, ActBF16, true>(a, s);
+  }
   if (state_dt == DT_BF16) return launch_recurrent<Act, ActBF16, GATE_F32>(a, s);
   if (state_dt == DT_F16) return launch_recurrent<Act, ActF16, GATE_F32>(a, s);
   return launch_recurrent<Act, ActF32, GATE_F32>(a, s);
 }
 
 }  // namespace
+
+int64_t prefill_work_bytes(int64_t T, int64_t N, int32_t H, int32_t HV, int act_dt, int state_dt) {
+  if (!chunked_form(T, N)) return 0;
+  const bool split = needs_split(act_dt, state_dt);
+  return (T / C + N) * (H * unit_bytes(split) + HV * head_bytes(split));
+}
 
 int launch_prefill(const PrefillArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream) {
   hipStream_t s = (hipStream_t)stream;
