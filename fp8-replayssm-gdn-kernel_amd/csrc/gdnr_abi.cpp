@@ -9,6 +9,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <string>
 #include <utility>
@@ -1428,6 +1429,8 @@ int gdnr_prefill(const gdnr_tensor* mixed_qkv, const gdnr_tensor* a, const gdnr_
   GDNR_TRY(check_act_tensor(out, "out", 3, {T, HV, V}, act, 16));
   GDNR_TRY(check_tokens(T, N));
   if (HV * V > INT32_MAX / 4 || S > INT32_MAX) return fail(GDNR_ERR_UNSUPPORTED, "state extents too large");
+  if (std::max(mixed_qkv->strides[0], out->strides[0]) > (1 << 23))
+    return fail(GDNR_ERR_UNSUPPORTED, "mixed_qkv and out: rows of more than 2^23 elements");
   if (N * HV * V == 0) return GDNR_OK;
   GDNR_TRY(check_workspace(workspace, gdnr_prefill_workspace(T, N, (int32_t)H, (int32_t)HV, (int32_t)V, act, state->dtype)));
   gdnr::PrefillArgs r = {};

@@ -76,25 +76,6 @@ __device__ __forceinline__ const StepArgs& opaque_args() {
   asm volatile("" : "+s"(lo), "+s"(hi));
   return *(const StepArgs*)(c_args*)(((uint64_t)hi << 32) | lo);
 }
-// Direct global -> LDS copy of 16 bytes per lane (global_load_lds_dwordx4):
-// lane l's 16 bytes land at LDS address lds_addr + 16 l (lds_addr wave-uniform,
-// through M0, which is restored). Written as inline assembly so that the
-// compiler does not order every later LDS read after it: the caller waits for
-// it (vmcnt) before reading the destination, and the compiler's own vmcnt
-// waits, which do not count it, can only wait longer than they need.
-__device__ __forceinline__ void dma16(const uint8_t* src, uint32_t lds_addr) {
-  uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %2, off\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(lds_addr), "v"(src)
-      : "memory");
-}
-
 // The U~ operand of a flush's K^T U~ MFMA (16x16x32, k-slot 8 q4 + j) from
 // this lane's 16-bit hi and lo words of tokens 4 q4 .. 4 q4 + 3 (h01 = hi
 // of tokens 4 q4 and 4 q4 + 1, ...). One half-wave swap per word pair gives

@@ -301,6 +301,40 @@ __device__ __forceinline__ bool wait_count(int* f, int target, uint32_t* status,
   return false;
 }
 
+// ---------------------------------------------------------------- global -> LDS
+// Direct global -> LDS copy of 16 bytes per lane (global_load_lds_dwordx4):
+// lane l's 16 bytes land at LDS address lds_addr + 16 l (lds_addr wave-uniform,
+// through M0, which is restored). Written as inline assembly so that the
+// compiler does not order every later LDS read after it: the caller waits for
+// it (vmcnt) before reading the destination, and the compiler's own vmcnt
+// waits, which do not count it, can only wait longer than they need.
+__device__ __forceinline__ void dma16(const uint8_t* src, uint32_t lds_addr) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds_addr), "v"(src)
+      : "memory");
+}
+
+// The same from a wave-uniform base and a 32-bit byte offset per lane.
+__device__ __forceinline__ void dma16_at(const uint8_t* base, uint32_t offset, uint32_t lds_addr) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, %3\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds_addr), "v"(offset), "s"(base)
+      : "memory");
+}
+
 // ---------------------------------------------------------------- waits
 // s_waitcnt immediate (gfx9): vmcnt[3:0] + vmcnt_hi[15:14], expcnt[6:4], lgkmcnt[11:8].
 #define GDNR_WAIT_VMCNT(n) \

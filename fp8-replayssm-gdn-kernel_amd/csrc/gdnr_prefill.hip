@@ -241,9 +241,10 @@ __device__ __forceinline__ f32x4_t product(const Operand<SPLIT>& a, const Operan
 // Workspace: per chunk slot and key head the unit keys and queries [C][K] f16
 // (SPLIT: high, then low); per slot and value head the operand tiles of T - I
 // and A (64 lanes x 16 bytes each; SPLIT: high, then low) and the tokens'
-// {beta}[C], {e^G}[C], {e^(G_C - G)}[C], first bad token (as an int), pad[3].
+// {beta}[C], {e^G}[C], {e^(G_C - G)}[C], the first bad token (an int), padded
+// to 1 KiB.
 // Sequence n's chunks take the slots from cu[n] / C + n on.
-constexpr int kScalars = 3 * C + 4;
+constexpr int kScalars = 256;
 __host__ __device__ constexpr int64_t unit_bytes(bool split) { return 2 * C * K * 2 * (split ? 2 : 1); }
 __host__ __device__ constexpr int64_t tile_bytes(bool split) { return 2 * kTri * 1024 * (split ? 2 : 1); }
 __host__ __device__ constexpr int64_t head_bytes(bool split) { return tile_bytes(split) + kScalars * 4; }
@@ -263,10 +264,13 @@ __host__ __device__ constexpr int scan_buffers(bool split) { return split ? 1 : 
 // index of the tile (16 rows of t, 32 columns of i) in a lower triangle
 __host__ __device__ constexpr int tri(int tt, int ts) { return tt < 2 ? tt : 2 * (tt - 1) + ts; }
 
-__device__ __forceinline__ float exp_diff(double d) {
-  const float h = (float)d;
-  const float e = expf(h);
-  return fmaf(e, (float)(d - (double)h), e);
+// 2^d of a difference of sums of log2 decays; SPLIT: with what rounding the
+// exponent to f32 leaves out
+template <bool SPLIT>
+__device__ __forceinline__ float exp2_diff(double d) {
+  const float h = (float)d, e = __builtin_amdgcn_exp2f(h);
+  if constexpr (!SPLIT) return e;
+  return fmaf(e, 0.6931471805599453f * (float)(d - (double)h), e);
 }
 
 // One chunk of one key head: 4 waves. The Gram products are formed transposed
@@ -278,7 +282,7 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
   constexpr int ES = Act::kBytes, RS = 2 * K + 16, P = SPLIT ? 2 : 1;  // LDS row of a key or query, halves
   constexpr int kUnits = 2 * P * C * RS, MS = 68 * 4, kM = C * MS;      // [i][t] f32 of M, per head
   __shared__ __attribute__((aligned(16))) uint8_t lds[kUnits > 2 * kM ? kUnits : 2 * kM];
-  __shared__ double Gs[2][C];
+  __shared__ double Gs[2][C];  // sums of log2 decays
   __shared__ float betas[2][C];
   __shared__ int bad_key;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -371,7 +375,7 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
       const int first = bads ? __ffsll((unsigned long long)bads) - 1 : C;
       if (t >= first) g = 0.f, beta = 0.f;
       // (a decay of e^-1e4 is 0 in every format; a sum of such stays exact)
-      double G = fmaxf(g, -1e4f);
+      double G = (double)fmaxf(g, -1e4f) * 1.4426950408889634;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) {
         const double up = __shfl_up(G, d);
@@ -382,8 +386,8 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
       betas[wave][t] = beta;
       float* sc = (float*)(w.head + ((int64_t)slot * a.HV + hv) * head_bytes(SPLIT) + tile_bytes(SPLIT));
       sc[t] = beta;
-      sc[C + t] = exp_diff(G);
-      sc[2 * C + t] = exp_diff(last - G);
+      sc[C + t] = exp2_diff<SPLIT>(G);
+      sc[2 * C + t] = exp2_diff<SPLIT>(last - G);
       if (t == 0) ((int*)sc)[3 * C] = first;
     }
     __syncthreads();
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 16 * c + 4 * grp + j;
-          const float decay = i <= t ? exp_diff(Gt - Gs[e][i]) : 0.f;
+          const float decay = i <= t ? exp2_diff<SPLIT>(Gt - Gs[e][i]) : 0.f;
           at[c][j] = i <= t ? decay * qk[c][j] : 0.f;
           *(float*)(lds + e * kM + i * MS + t * 4) = i < t ? bt * decay * kk[c][j] : 0.f;
         }
@@ -415,39 +419,69 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
       }
     }
     __syncthreads();
-    if (wave < heads) {
-      // row t of T, one lane each: x (I + M) = e_t, from the last column on
-      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + wave) * head_bytes(SPLIT);
-      const uint8_t* m = lds + wave * kM;
-      float x[C];
+    // T = (I + M)^-1 by blocks of 16, wave w the block row w. First its
+    // diagonal block, a lane a row of it (lanes of group e: head g0 + e): from
+    // x (I + M) = e_t, the last column first. It takes M's place.
+    if (grp < heads) {
+      uint8_t* m = lds + grp * kM + 16 * wave * (MS + 4);
+      f32x4_t row[16][4];
 #pragma unroll
-      for (int i = C - 1; i >= 0; --i) {
-        float acc[2] = {lane == i ? 1.f : 0.f, 0.f};
+      for (int i = 0; i < 16; ++i)
 #pragma unroll
-        for (int j0 = (i + 1) & ~3; j0 < C; j0 += 4) {
-          const f32x4_t mj = *(const f32x4_t*)(m + i * MS + j0 * 4);
+        for (int j = (i + 1) / 4; j < 4; ++j) row[i][j] = *(const f32x4_t*)(m + i * MS + 16 * j);
+      float x[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j0 + j > i) acc[j & 1] = fmaf(-x[j0 + j], mj[j], acc[j & 1]);
-        }
-        x[i] = acc[0] + acc[1];
+      for (int i = 15; i >= 0; --i) {
+        x[i] = col == i ? 1.f : 0.f;
+#pragma unroll
+        for (int j = 15; j > i; --j) x[i] = fmaf(-x[j], row[i][j >> 2][j & 3], x[i]);
       }
 #pragma unroll
-      for (int i = 0; i < C; ++i) x[i] = lane == i ? 0.f : SPLIT ? x[i] * kFix : x[i];  // T - I
-      const int tt = lane >> 4;
+      for (int i = 0; i < 16; ++i) *(float*)(m + i * MS + 4 * col) = x[i];
+    }
+    __syncthreads();
+    // Then T_wJ = -(sum over L = J+1..w of T_wL M_LJ) T_JJ, the nearest block
+    // first, transposed (rows of J on registers, t on lanes): what one product
+    // leaves is the next one's right operand, and M and T_JJ are read from LDS
+    // as they lie.
+    for (int e = 0; e < heads; ++e) {
+      const uint8_t* m = lds + e * kM;
+      f32x4_t x[4];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (2 * s <= tt) {
+      for (int c = 3; c >= 0; --c) {
+        x[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (c == wave)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int i = 32 * s + 4 * g;
-            const Operand<SPLIT> o = operand<SPLIT>(f32x4_t{x[i], x[i + 1], x[i + 2], x[i + 3]},
-                                                    f32x4_t{x[i + 16], x[i + 17], x[i + 18], x[i + 19]});
-            uint8_t* p = tiles + tri(tt, s) * 1024 + 16 * (16 * g + col);
-            *(u32x4_t*)p = o.hi;
-            if constexpr (SPLIT) *(u32x4_t*)(p + kTri * 1024) = o.lo;
-          }
+          for (int j = 0; j < 4; ++j) x[c][j] = *(const float*)(m + (16 * c + 4 * grp + j) * MS + (16 * c + col) * 4);
+        if (c >= wave) continue;
+        f32x4_t y = x[c];
+#pragma unroll
+        for (int l = c + 1; l < 4; ++l) {
+          if (l > wave) continue;
+          const f32x4_t ml = *(const f32x4_t*)(m + (16 * c + col) * MS + (16 * l + 4 * grp) * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y = __builtin_amdgcn_mfma_f32_16x16x4f32(ml[j], x[l][j], y, 0, 0, 0);
         }
+        const f32x4_t tl = *(const f32x4_t*)(m + (16 * c + col) * MS + (16 * c + 4 * grp) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(-tl[j], y[j], x[c], 0, 0, 0);
+      }
+      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + e) * head_bytes(SPLIT);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (c == wave && 4 * grp + j == col) x[c][j] = 0.f;  // T - I
+          if constexpr (SPLIT) x[c][j] *= kFix;
+        }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (2 * s > wave) continue;
+        const Operand<SPLIT> o = operand<SPLIT>(x[2 * s], x[2 * s + 1]);
+        uint8_t* p = tiles + tri(wave, s) * 1024 + 16 * lane;
+        *(u32x4_t*)p = o.hi;
+        if constexpr (SPLIT) *(u32x4_t*)(p + kTri * 1024) = o.lo;
+      }
     }
   }
 }
@@ -455,8 +489,10 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 // over the lanes of one column (lane & 15), in each of them
 __device__ __forceinline__ uint32_t column_max(uint32_t x) {
-  x = max(x, (uint32_t)__shfl_xor((int)x, 16));
-  return max(x, (uint32_t)__shfl_xor((int)x, 32));
+  const auto half = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = max(half[0], half[1]);
+  const auto row = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max(row[0], row[1]);
 }
 
 // A sequence's chunks in order, for 16 NV V-rows of one value head a wave,
@@ -466,9 +502,9 @@ __device__ __forceinline__ uint32_t column_max(uint32_t x) {
 // operand as it stands: both operands of a product may take its contraction in
 // any order, and the keys', T's and A's fragments are read in that one.
 template <class Act, class St, bool SPLIT, int WAVES, int NV>
-__global__ __launch_bounds__(64 * WAVES) void chunk_scan_kernel(const PrefillArgs a) {
-  constexpr int ES = Act::kBytes, P = SPLIT ? 2 : 1, RS = 2 * K + 32;  // LDS row: 16 rows' 32-byte pieces on distinct banks
-  constexpr int THREADS = 64 * WAVES, kUnitRows = 2 * P * C, kUnits = kUnitRows * RS;
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_scan_kernel(const PrefillArgs a) {
+  constexpr int ES = Act::kBytes, P = SPLIT ? 2 : 1, RS = 2 * K;
+  constexpr int kUnits = 2 * P * C * RS;
   constexpr int kHead = (int)head_bytes(SPLIT), kBuf = kUnits + kHead;
   constexpr int BUFS = scan_buffers(SPLIT);
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -482,8 +518,14 @@ __global__ __launch_bounds__(64 * WAVES) void chunk_scan_kernel(const PrefillArg
   sequence_rows(a, n, begin, end);
   const bool started = sequence_started(a, n);
   if (begin == end && started) return;
-  const Work w = work_of(a, SPLIT);
-  const int slot0 = begin / C + n, chunks = (end - begin + C - 1) / C;
+  const int len = end - begin, chunks = (len + C - 1) / C;
+  const uint8_t *unit, *head;  // of the next chunk to fetch
+  {
+    const Work w = work_of(a, SPLIT);
+    const int64_t slot0 = begin / C + n;
+    unit = w.unit + (slot0 * a.H + h) * unit_bytes(SPLIT);
+    head = w.head + (slot0 * a.HV + hv) * head_bytes(SPLIT);
+  }
 
   // the state, transposed: tile kt of 16 columns k, rows 4 grp + j
   uint8_t* sp = (uint8_t*)a.state + ((int64_t)sequence_slot(a, n) * a.st_s + hv * a.st_h + (int64_t)v0 * a.st_v + 4 * grp) * St::kBytes;
@@ -501,63 +543,132 @@ __global__ __launch_bounds__(64 * WAVES) void chunk_scan_kernel(const PrefillArg
     }
   }
 
-  // a chunk's operands: global -> registers (while the chunk before is
-  // computed) -> LDS
-  constexpr int kPieces = (kUnitRows * 16 + kHead / 16 + THREADS - 1) / THREADS;
-  u32x4_t piece[kPieces];
+  // a chunk's operands, straight from memory to LDS, 1 KiB an instruction. Row
+  // r keeps its 16-byte piece p at p ^ (r & 15): the 16 rows of a fragment's
+  // read then lie on distinct banks.
+  constexpr int kRowPieces = kUnits / 1024, kPieces = kRowPieces + kHead / 1024;
+  static_assert(kRowPieces % (4 * WAVES) == 0, "a wave's row pieces come in fours");
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds;
+  uint32_t row_off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row_off[i] = 1024 * i + 256 * grp + 16 * (col ^ (4 * i + grp));
   auto fetch = [&](int c) {
-    const uint8_t* unit = w.unit + ((int64_t)(slot0 + c) * a.H + h) * unit_bytes(SPLIT);
-    const uint8_t* head = w.head + ((int64_t)(slot0 + c) * a.HV + hv) * head_bytes(SPLIT);
+    const uint32_t to = lds0 + (uint32_t)((c % BUFS) * kBuf);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int x = i * THREADS + (int)threadIdx.x;
-      if (x < kUnitRows * 16) piece[i] = *(const u32x4_t*)(unit + 16 * x);
-      else if (x < kUnitRows * 16 + kHead / 16) piece[i] = *(const u32x4_t*)(head + 16 * (x - kUnitRows * 16));
+    for (int i = 0; i < kRowPieces / WAVES; ++i) {
+      const int x = (i & ~3) * WAVES + 4 * wave;
+      dma16_at(unit + x * 1024, row_off[i & 3], to + (x + (i & 3)) * 1024);
     }
-  };
-  auto stage = [&](int c) {
-    uint8_t* b = lds + (c % BUFS) * kBuf;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int x = i * THREADS + (int)threadIdx.x;
-      if (x < kUnitRows * 16) *(u32x4_t*)(b + (x >> 4) * RS + 16 * (x & 15)) = piece[i];
-      else if (x < kUnitRows * 16 + kHead / 16) *(u32x4_t*)(b + kUnits + 16 * (x - kUnitRows * 16)) = piece[i];
+    for (int i = 0; i < (kHead / 1024 + WAVES - 1) / WAVES; ++i) {
+      const int x = i * WAVES + wave;  // wave-uniform
+      if (x < kHead / 1024) dma16_at(head + x * 1024, 16 * lane, to + kUnits + x * 1024);
     }
+    unit += a.H * unit_bytes(SPLIT), head += a.HV * head_bytes(SPLIT);
   };
-  // the chunk's v: rows t of this lane, NV neighbours each
-  float vn[NV][4][4];
-  const uint8_t* vp = (const uint8_t*)a.mixed + (2 * a.H * K + (int64_t)hv * a.V + v0) * ES;
+  // the chunk's v: rows t of this lane, NV neighbours each, as raw bits
+  using VBits = typename std::conditional<NV == 2, typename Act::Pair, typename Act::Bits>::type;
+  VBits vn[16];
+  const int64_t v_row = a.mx_t * ES, o_row = a.o_t * ES;
+  const uint8_t* vp = (const uint8_t*)a.mixed + (int64_t)begin * v_row + (2 * a.H * K + hv * a.V) * ES;
+  uint8_t* op = (uint8_t*)a.out + (int64_t)begin * o_row + hv * a.o_h * ES;
+  const uint32_t v_lane = (uint32_t)(4 * grp * v_row) + v0 * ES, o_lane = (uint32_t)(4 * grp * o_row) + v0 * ES;
+  auto load_v = [&](int i, const uint8_t* p) {
+    if constexpr (NV == 2) vn[i] = Act::ld_pair_bits(p);
+    else vn[i] = Act::ld_bits(p, 0);
+  };
   auto fetch_v = [&](int c) {
+    const uint8_t* p = vp + c * C * v_row;
+    if ((c + 1) * C <= len) {
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
+      for (int i = 0; i < 16; ++i) load_v(i, p + (16 * (i >> 2) + (i & 3)) * v_row + v_lane);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = c * C + 16 * tt + 4 * grp + j;
-        const bool on = begin + t < end;
-        const uint8_t* p = vp + (int64_t)min(begin + t, end - 1) * a.mx_t * ES;
-        if constexpr (NV == 2) {
-          const float2 x = Act::ld2(p);
-          vn[0][tt][j] = on ? x.x : 0.f, vn[1][tt][j] = on ? x.y : 0.f;
-        } else {
-          const float x = Act::ld(p, 0);
-          vn[0][tt][j] = on ? x : 0.f;
-        }
-      }
+      for (int i = 0; i < 16; ++i) load_v(i, p + (uint32_t)min(16 * (i >> 2) + (i & 3) + 4 * grp, len - 1 - c * C) * v_row + v0 * ES);
+    }
   };
 
-  if (chunks) fetch(0), fetch_v(0), stage(0);
+  if (chunks) {
+    fetch(0), fetch_v(0);
+    GDNR_WAIT_VMCNT(0);
+  }
   for (int c = 0; c < chunks; ++c) {
-    __syncthreads();  // chunk c's operands are in LDS; those of c - 1 are no longer read
+    // chunk c's operands are in LDS (every wave waited for its part), those of
+    // c - 1 are no longer read
+    __syncthreads();
     const uint8_t* b = lds + (c % BUFS) * kBuf;
-    const uint8_t* head = b + kUnits;
-    const float* scal = (const float*)(head + tile_bytes(SPLIT));
+    const uint8_t* tiles = b + kUnits;
+    const float* scal = (const float*)(tiles + tile_bytes(SPLIT));
+    auto rows_of = [&](int plane, int tile, int step) {  // 16 tokens by 32 columns k
+      Operand<SPLIT> o;
+      const uint8_t* p = b + (plane * C + 16 * tile + col) * RS + 8 * (grp & 1);
+      const int x = 16 * ((4 * step + (grp >> 1)) ^ col), y = x ^ 32;
+      const uint2 lo = *(const uint2*)(p + x), hi = *(const uint2*)(p + y);
+      o.hi = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+      if constexpr (SPLIT) {
+        const uint2 z = *(const uint2*)(p + C * RS + x), u = *(const uint2*)(p + C * RS + y);
+        o.lo = u32x4_t{z.x, z.y, u.x, u.y};
+      }
+      return o;
+    };
+    auto turned = [&](int tile, int step) {  // 16 columns k of the keys by 32 tokens
+      Operand<SPLIT> o;
+      const int row = 4 * grp + (col >> 2);
+      const uint8_t* p = b + (32 * step + row) * RS + 16 * ((2 * tile + ((col & 3) >> 1)) ^ row) + 8 * (col & 1);
+      auto read = [](const uint8_t* q) { return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q)); };
+      const uint2 x = read(p), y = read(p + 16 * RS);
+      o.hi = u32x4_t{x.x, x.y, y.x, y.y};
+      if constexpr (SPLIT) {
+        const uint2 z = read(p + C * RS), u = read(p + (C + 16) * RS);
+        o.lo = u32x4_t{z.x, z.y, u.x, u.y};
+      }
+      return o;
+    };
+    auto triangle = [&](int base, int tt, int ts) {
+      Operand<SPLIT> o;
+      const uint8_t* p = tiles + (base * P + tri(tt, ts)) * 1024 + 16 * lane;
+      o.hi = *(const u32x4_t*)p;
+      if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + kTri * 1024);
+      return o;
+    };
+    constexpr float kUp = SPLIT ? kFix : 1.f, kDown = 1.f / kUp;
+    const f32x4_t* beta4 = (const f32x4_t*)scal;
+    const f32x4_t* grow4 = (const f32x4_t*)(scal + C);
+    const f32x4_t* end4 = (const f32x4_t*)(scal + 2 * C);
+    const float total = scal[2 * C - 1];
+    const int bad_token = __builtin_amdgcn_readfirstlane(((const int*)scal)[3 * C]);
+
     float v[NV][4][4];
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv)
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (NV == 2) {
+        const float2 x = Act::from_pair(vn[i]);
+        v[0][i >> 2][i & 3] = x.x, v[1][i >> 2][i & 3] = x.y;
+      } else {
+        v[0][i >> 2][i & 3] = Act::from_bits(vn[i]);
+      }
+    }
+    if ((c + 1) * C > len) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[nv][i >> 2][i & 3] = vn[nv][i >> 2][i & 3];
-    if (c + 1 < chunks) fetch(c + 1), fetch_v(c + 1);
-    const int bad_token = __builtin_amdgcn_readfirstlane(((const int*)scal)[3 * C]);
+      for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c * C + 16 * (i >> 2) + 4 * grp + (i & 3) >= len) v[nv][i >> 2][i & 3] = 0.f;
+    }
+    if (c + 1 < chunks) {
+      if constexpr (BUFS == 2) fetch(c + 1);
+      fetch_v(c + 1);
+    }
+
+    constexpr int AHEAD = SPLIT ? 1 : 2;  // k-steps of 4 fragments read before the first product
+    Operand<SPLIT> f[AHEAD + 1][4];
+    auto read_rows = [&](int plane, int s) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) f[s % (AHEAD + 1)][tt] = rows_of(plane, tt, s);
+    };
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) read_rows(0, s);
+    GDNR_COMPILER_FENCE();
 
     // V-rows with a value that is not finite: zeros here, NaN from its token on
     uint32_t ms[NV], mv[NV];
@@ -598,6 +709,7 @@ __global__ __launch_bounds__(64 * WAVES) void chunk_scan_kernel(const PrefillArg
       }
     }
     // each row's power of two: |R| and |U| are at most 64 (|v| + 12 |S|)
+    Operand<SPLIT> bs[NV][4];
 #pragma unroll
     for (int nv = 0; nv < NV; ++nv) {
       const float bound = fmaxf(__uint_as_float(mv[nv]), 12.f * __uint_as_float(ms[nv]) * inv[nv]);
@@ -606,155 +718,169 @@ __global__ __launch_bounds__(64 * WAVES) void chunk_scan_kernel(const PrefillArg
 #pragma unroll
       for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= ratio;
       sc[nv] = s_new, inv[nv] = __uint_as_float((ex - 14u) << 23);
-    }
-
-    const f32x4_t* beta4 = (const f32x4_t*)scal;
-    const f32x4_t* grow4 = (const f32x4_t*)(scal + C);
-    const f32x4_t* end4 = (const f32x4_t*)(scal + 2 * C);
-    const float total = scal[2 * C - 1];
-    auto rows_of = [&](int plane, int tile, int step) {  // 16 tokens by 32 columns k
-      Operand<SPLIT> o;
-      const uint8_t* p = b + (plane * C + 16 * tile + col) * RS + 64 * step + 8 * grp;
-      const uint2 x = *(const uint2*)p, y = *(const uint2*)(p + 32);
-      o.hi = u32x4_t{x.x, x.y, y.x, y.y};
-      if constexpr (SPLIT) {
-        const uint2 z = *(const uint2*)(p + C * RS), u = *(const uint2*)(p + C * RS + 32);
-        o.lo = u32x4_t{z.x, z.y, u.x, u.y};
-      }
-      return o;
-    };
-    auto turned = [&](int tile, int step) {  // 16 columns k of the keys by 32 tokens
-      Operand<SPLIT> o;
-      const uint8_t* p = b + (32 * step + 4 * grp + (col >> 2)) * RS + 32 * tile + 8 * (col & 3);
-      auto read = [](const uint8_t* q) { return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q)); };
-      const uint2 x = read(p), y = read(p + 16 * RS);
-      o.hi = u32x4_t{x.x, x.y, y.x, y.y};
-      if constexpr (SPLIT) {
-        const uint2 z = read(p + C * RS), u = read(p + (C + 16) * RS);
-        o.lo = u32x4_t{z.x, z.y, u.x, u.y};
-      }
-      return o;
-    };
-    auto triangle = [&](int base, int tt, int ts) {
-      Operand<SPLIT> o;
-      const uint8_t* p = head + (base * P + tri(tt, ts)) * 1024 + 16 * lane;
-      o.hi = *(const u32x4_t*)p;
-      if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + kTri * 1024);
-      return o;
-    };
-    constexpr float kUp = SPLIT ? kFix : 1.f, kDown = 1.f / kUp;
-
-    Operand<SPLIT> bs[NV][4];
-#pragma unroll
-    for (int nv = 0; nv < NV; ++nv)
 #pragma unroll
       for (int s = 0; s < 4; ++s) bs[nv][s] = operand<SPLIT>(S[nv][2 * s], S[nv][2 * s + 1]);
-    // R = beta (v - e^G (K S0^T)), U = R + (T - I) R
-    f32x4_t u[NV][4];
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      f32x4_t x[NV];
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv) x[nv] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // The products. Their LDS operands are read a stage or more before they
+    // are used, which the fences keep the compiler from undoing: a read just
+    // before its product costs its latency some 60 times a chunk.
+    f32x4_t u[NV][4], o[NV][4];
+    auto by_state = [&](int plane, f32x4_t(&x)[NV][4]) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const Operand<SPLIT> k = rows_of(0, tt, s);
+        if (s + AHEAD < 4) read_rows(plane, s + AHEAD);
+        GDNR_COMPILER_FENCE();
 #pragma unroll
-        for (int nv = 0; nv < NV; ++nv) x[nv] = product<SPLIT>(k, bs[nv][s], x[nv]);
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int nv = 0; nv < NV; ++nv)
+            x[nv][tt] = product<SPLIT>(f[s % (AHEAD + 1)][tt], bs[nv][s], s == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[nv][tt]);
       }
-      const f32x4_t be = beta4[4 * tt + grp], gr = grow4[4 * tt + grp];
+    };
+    by_state(0, u);  // K S0^T (its first fragments were read at the top)
+    GDNR_COMPILER_FENCE();
+    Operand<SPLIT> tf[kTri];
+    auto read_triangle = [&](int base) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int s = 0; s <= tt / 2; ++s) tf[tri(tt, s)] = triangle(base, tt, s);
+    };
+    f32x4_t be[4], gr[4];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) be[tt] = beta4[4 * tt + grp], gr[tt] = grow4[4 * tt + grp];
+    if constexpr (!SPLIT) read_triangle(0);
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) read_rows(P, s);
+    GDNR_COMPILER_FENCE();
+    // R = beta (v - e^G (K S0^T))
+    Operand<SPLIT> ub[NV][2], ud[NV][2];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
       for (int nv = 0; nv < NV; ++nv)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[nv][tt][j] = be[j] * (v[nv][tt][j] * sc[nv] - gr[j] * kDown * x[nv][j]);
-    }
-    Operand<SPLIT> ub[NV][2], ud[NV][2];
+        for (int j = 0; j < 4; ++j) u[nv][tt][j] = be[tt][j] * (v[nv][tt][j] * sc[nv] - gr[tt][j] * kDown * u[nv][tt][j]);
 #pragma unroll
     for (int nv = 0; nv < NV; ++nv)
 #pragma unroll
       for (int s = 0; s < 2; ++s) ub[nv][s] = operand<SPLIT>(u[nv][2 * s], u[nv][2 * s + 1]);
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
+    // U = R + (T - I) R
+    if constexpr (SPLIT) {
+      read_triangle(0);
 #pragma unroll
       for (int nv = 0; nv < NV; ++nv)
-        if constexpr (SPLIT) u[nv][tt] *= kUp;
 #pragma unroll
-      for (int s = 0; s <= tt / 2; ++s) {
-        const Operand<SPLIT> m = triangle(0, tt, s);
+        for (int tt = 0; tt < 4; ++tt) u[nv][tt] *= kUp;
+    }
 #pragma unroll
-        for (int nv = 0; nv < NV; ++nv) u[nv][tt] = product<SPLIT>(m, ub[nv][s], u[nv][tt]);
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int tt = 2 * s; tt < 4; ++tt)
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) u[nv][tt] = product<SPLIT>(tf[tri(tt, s)], ub[nv][s], u[nv][tt]);
+    by_state(P, o);  // Q S0^T
+    GDNR_COMPILER_FENCE();
+    f32x4_t ed[4];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) ed[tt] = end4[4 * tt + grp];
+    constexpr int KT = SPLIT ? 2 : 4;  // tiles of the keys read ahead
+    Operand<SPLIT> kf[2][KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) kf[0][kt] = turned(kt, 0);
+    if constexpr (!SPLIT) read_triangle(kTri);
+    GDNR_COMPILER_FENCE();
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv) {
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) u[nv][tt] *= kDown;
       }
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-        if constexpr (SPLIT) u[nv][tt] *= kDown;
+      for (int s = 0; s < 2; ++s) {
+        ud[nv][s] = operand<SPLIT>(u[nv][2 * s] * ed[2 * s], u[nv][2 * s + 1] * ed[2 * s + 1]);
+        ub[nv][s] = operand<SPLIT>(u[nv][2 * s], u[nv][2 * s + 1]);
+      }
     }
+    // the state after the chunk
 #pragma unroll
     for (int nv = 0; nv < NV; ++nv)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        ub[nv][s] = operand<SPLIT>(u[nv][2 * s], u[nv][2 * s + 1]);
-        ud[nv][s] = operand<SPLIT>(u[nv][2 * s] * end4[8 * s + grp], u[nv][2 * s + 1] * end4[8 * s + 4 + grp]);
+      for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= total * kUp;
+#pragma unroll
+    for (int i = 0; i < 16 / KT; ++i) {  // KT tiles of one half of the tokens at a time
+      if (i + 1 < 16 / KT) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) kf[(i + 1) & 1][kt] = turned(((i + 1) * KT + kt) % 8, (i + 1) * KT / 8);
       }
-    // the state after the chunk
+      GDNR_COMPILER_FENCE();
 #pragma unroll
-    for (int kt = 0; kt < 8; ++kt) {
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv) S[nv][kt] *= total * kUp;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const Operand<SPLIT> k = turned(kt, s);
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) S[nv][kt] = product<SPLIT>(k, ud[nv][s], S[nv][kt]);
-      }
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-        if constexpr (SPLIT) S[nv][kt] *= kDown;
-    }
-    // the outputs
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      f32x4_t o[NV];
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv) o[nv] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const Operand<SPLIT> q = rows_of(P, tt, s);
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) o[nv] = product<SPLIT>(q, bs[nv][s], o[nv]);
-      }
-      const f32x4_t gr = grow4[4 * tt + grp];
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv) o[nv] *= gr;
-#pragma unroll
-      for (int s = 0; s <= tt / 2; ++s) {
-        const Operand<SPLIT> m = triangle(kTri, tt, s);
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) o[nv] = product<SPLIT>(m, ub[nv][s], o[nv]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 16 * tt + 4 * grp + j;
-        if (c * C + t >= end - begin) continue;
-        uint8_t* p = (uint8_t*)a.out + ((int64_t)(begin + c * C + t) * a.o_t + hv * a.o_h + v0) * ES;
-        float y[NV];
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int nv = 0; nv < NV; ++nv) {
-          y[nv] = o[nv][j] * kDown * (a.out_scale * inv[nv]);
-          if (any_bad && t >= first[nv]) y[nv] = __builtin_nanf("");
+          f32x4_t& x = S[nv][(i * KT + kt) % 8];
+          x = product<SPLIT>(kf[i & 1][kt], ud[nv][i * KT / 8], x);
         }
-        if constexpr (NV == 2) Act::st2(p, y[0], y[1]);
-        else Act::st(p, 0, y[0]);
-      }
+    }
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+        for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= kDown;
+    }
+    // the outputs
+    if constexpr (SPLIT) read_triangle(kTri);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) o[nv][tt] *= gr[tt];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int tt = 2 * s; tt < 4; ++tt)
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) o[nv][tt] = product<SPLIT>(tf[tri(tt, s)], ub[nv][s], o[nv][tt]);
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv) {
+      const float f = kDown * a.out_scale * inv[nv];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) o[nv][tt] *= f;
     }
     if (any_bad) {
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-        if (first[nv] < C)
+      for (int nv = 0; nv < NV; ++nv) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (16 * (i >> 2) + 4 * grp + (i & 3) >= first[nv]) o[nv][i >> 2][i & 3] = __builtin_nanf("");
+        if (first[nv] < C) {
 #pragma unroll
           for (int kt = 0; kt < 8; ++kt) S[nv][kt] = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+        }
+      }
     }
-    if constexpr (BUFS == 1) __syncthreads();
-    if (c + 1 < chunks) stage(c + 1);
+    // (the next chunk's operands are waited for before the stores, which then
+    // have a whole chunk to drain)
+    if (BUFS == 2) GDNR_WAIT_VMCNT(0);
+    uint8_t* orow = op + c * C * o_row;
+    auto store_o = [&](int i) {
+      uint8_t* p = orow + (16 * (i >> 2) + (i & 3)) * o_row + o_lane;
+      if constexpr (NV == 2) Act::st2(p, o[0][i >> 2][i & 3], o[1][i >> 2][i & 3]);
+      else Act::st(p, 0, o[0][i >> 2][i & 3]);
+    };
+    if ((c + 1) * C <= len) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) store_o(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c * C + 16 * (i >> 2) + (i & 3) + 4 * grp < len) store_o(i);
+    }
+    if (BUFS == 1 && c + 1 < chunks) {
+      __syncthreads();
+      fetch(c + 1);
+      GDNR_WAIT_VMCNT(0);
+    }
   }
 #pragma unroll
   for (int nv = 0; nv < NV; ++nv)
@@ -778,7 +904,7 @@ int launch_prep(const PrefillArgs& a, hipStream_t s) {
 }
 template <class Act, class St, bool SPLIT, int WAVES, int NV>
 int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
-  constexpr int lds = scan_buffers(SPLIT) * (2 * (SPLIT ? 2 : 1) * C * (2 * K + 32) + (int)head_bytes(SPLIT));
+  constexpr int lds = scan_buffers(SPLIT) * (2 * (SPLIT ? 2 : 1) * C * 2 * K + (int)head_bytes(SPLIT));
   static_assert(lds <= kMaxStepLds, "the operands fit");
   const auto kernel = chunk_scan_kernel<Act, St, SPLIT, WAVES, NV>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
