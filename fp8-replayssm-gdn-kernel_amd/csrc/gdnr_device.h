@@ -321,18 +321,37 @@ __device__ __forceinline__ void dma16(const uint8_t* src, uint32_t lds_addr) {
       : "memory");
 }
 
-// The same from a wave-uniform base and a 32-bit byte offset per lane.
-__device__ __forceinline__ void dma16_at(const uint8_t* base, uint32_t offset, uint32_t lds_addr) {
+// 1024 N consecutive bytes at `src` (wave-uniform) to LDS address lds_addr, 1 KiB
+// an instruction (its immediate offset counts in both addresses).
+template <int N>
+__device__ __forceinline__ void dma_kib(const uint8_t* src, uint32_t lds_addr) {
+  static_assert(N == 2 || N == 4, "pieces of 2 or 4 KiB");
+  const uint32_t offset = 16 * (threadIdx.x & 63);
   uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %2, %3\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(lds_addr), "v"(offset), "s"(base)
-      : "memory");
+  if constexpr (N == 4)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, %3\n\t"
+        "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
+        "global_load_lds_dwordx4 %2, %3 offset:2048\n\t"
+        "global_load_lds_dwordx4 %2, %3 offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(lds_addr), "v"(offset), "s"(src)
+        : "memory");
+  else
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, %3\n\t"
+        "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(lds_addr), "v"(offset), "s"(src)
+        : "memory");
 }
 
 // ---------------------------------------------------------------- waits

@@ -239,15 +239,15 @@ __device__ __forceinline__ f32x4_t product(const Operand<SPLIT>& a, const Operan
 }
 
 // Workspace: per chunk slot and key head the unit keys and queries [C][K] f16
-// (SPLIT: high, then low); per slot and value head the operand tiles of T - I
+// (SPLIT: high, then low), a row's pieces as unit_at places them; per slot and value head the operand tiles of T - I
 // and A (64 lanes x 16 bytes each; SPLIT: high, then low) and the tokens'
-// {beta}[C], {e^G}[C], {e^(G_C - G)}[C], the first bad token (an int), padded
-// to 1 KiB.
+// {beta}[C], {e^G}[C], {e^(G_C - G)}[C], {-beta e^G}[C], first bad token (an
+// int), padded to 2 KiB.
 // Sequence n's chunks take the slots from cu[n] / C + n on.
-constexpr int kScalars = 256;
+constexpr int kScalars = 4 * C + 4;
 __host__ __device__ constexpr int64_t unit_bytes(bool split) { return 2 * C * K * 2 * (split ? 2 : 1); }
 __host__ __device__ constexpr int64_t tile_bytes(bool split) { return 2 * kTri * 1024 * (split ? 2 : 1); }
-__host__ __device__ constexpr int64_t head_bytes(bool split) { return tile_bytes(split) + kScalars * 4; }
+__host__ __device__ constexpr int64_t head_bytes(bool split) { return tile_bytes(split) + 2048; }
 
 struct Work {
   uint8_t* unit;  // [slots][H]
@@ -256,6 +256,14 @@ struct Work {
 __host__ __device__ inline Work work_of(const PrefillArgs& a, bool split) {
   const int64_t slots = a.T / C + a.N;
   return {a.work, a.work + slots * a.H * unit_bytes(split)};
+}
+
+// Byte of 4 elements (k = 4 k4 ..) of row t. A 16-byte piece holds the 8 elements
+// that a lane gives to a product over 32 columns (4 g .. + 3 of each half of
+// them), and row t keeps its piece p at p ^ (t & 15), so that the 16 rows of a
+// fragment lie on distinct LDS banks.
+__host__ __device__ constexpr int unit_at(int t, int k4) {
+  return 2 * K * t + 16 * ((4 * (k4 >> 3) + (k4 & 3)) ^ (t & 15)) + 8 * ((k4 >> 2) & 1);
 }
 
 // chunks whose operands the scan keeps in LDS
@@ -328,10 +336,12 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
     const Operand<SPLIT> o = operand<SPLIT>(f32x4_t{x[0] * f, x[1] * f, x[2] * f, x[3] * f}, f32x4_t{x[4] * f, x[5] * f, x[6] * f, x[7] * f});
     const int plane = (is_q ? P : 0);
     *(u32x4_t*)(lds + (plane * C + t) * RS + 16 * col) = o.hi;
-    *(u32x4_t*)(unit + (plane * C + t) * (2 * K) + 16 * col) = o.hi;
+    *(uint2*)(unit + plane * C * 2 * K + unit_at(t, 2 * col)) = make_uint2(o.hi[0], o.hi[1]);
+    *(uint2*)(unit + plane * C * 2 * K + unit_at(t, 2 * col + 1)) = make_uint2(o.hi[2], o.hi[3]);
     if constexpr (SPLIT) {
       *(u32x4_t*)(lds + ((plane + 1) * C + t) * RS + 16 * col) = o.lo;
-      *(u32x4_t*)(unit + ((plane + 1) * C + t) * (2 * K) + 16 * col) = o.lo;
+      *(uint2*)(unit + (plane + 1) * C * 2 * K + unit_at(t, 2 * col)) = make_uint2(o.lo[0], o.lo[1]);
+      *(uint2*)(unit + (plane + 1) * C * 2 * K + unit_at(t, 2 * col + 1)) = make_uint2(o.lo[2], o.lo[3]);
     }
   }
   __syncthreads();
@@ -388,7 +398,8 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
       sc[t] = beta;
       sc[C + t] = exp2_diff<SPLIT>(G);
       sc[2 * C + t] = exp2_diff<SPLIT>(last - G);
-      if (t == 0) ((int*)sc)[3 * C] = first;
+      sc[3 * C + t] = -beta * exp2_diff<SPLIT>(G) * (SPLIT ? 1.f / kFix : 1.f);
+      if (t == 0) ((int*)sc)[4 * C] = first;
     }
     __syncthreads();
     for (int e = 0; e < heads; ++e) {
@@ -486,13 +497,18 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
   }
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
-// over the lanes of one column (lane & 15), in each of them
-__device__ __forceinline__ uint32_t column_max(uint32_t x) {
-  const auto half = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  x = max(half[0], half[1]);
-  const auto row = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  return max(row[0], row[1]);
+// max(m, |a|, |b|), NaN propagating (one v_maximum3_f32)
+__device__ __forceinline__ float max3_abs(float m, float a, float b) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, __builtin_fabsf(a)), __builtin_fabsf(b));
+}
+__device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
+// over the lanes of one column (lane & 15), in each of them; NaN propagating
+__device__ __forceinline__ float column_max(float x) {
+  const uint32_t b = __float_as_uint(x);
+  const auto half = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t h = __float_as_uint(__builtin_elementwise_maximum(__uint_as_float(half[0]), __uint_as_float(half[1])));
+  const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(row[0]), __uint_as_float(row[1]));
 }
 
 // A sequence's chunks in order, for 16 NV V-rows of one value head a wave,
@@ -511,8 +527,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   constexpr int COLS = 16 * NV * WAVES;
-  const int blocks = a.V / COLS, hv = blockIdx.x / blocks, n = blockIdx.y;
-  const int v0 = (blockIdx.x - hv * blocks) * COLS + wave * 16 * NV + col * NV;  // this lane's V-rows: v0 .. v0 + NV - 1
+  // Workgroups go to the 8 XCDs in turn: those of one key head, which read the
+  // same keys and queries, to one of them.
+  const int blocks = a.V / COLS, n = blockIdx.y;
+  int unit_id = blockIdx.x;
+  if (a.H % 8 == 0) {
+    const int per = a.G * blocks, j = unit_id >> 3;
+    unit_id = ((unit_id & 7) + 8 * (j / per)) * per + j % per;
+  }
+  const int hv = unit_id / blocks;
+  const int v0 = (unit_id - hv * blocks) * COLS + wave * 16 * NV + col * NV;  // this lane's V-rows: v0 .. v0 + NV - 1
   const int h = hv / a.G;
   int begin, end;
   sequence_rows(a, n, begin, end);
@@ -543,26 +567,19 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     }
   }
 
-  // a chunk's operands, straight from memory to LDS, 1 KiB an instruction. Row
-  // r keeps its 16-byte piece p at p ^ (r & 15): the 16 rows of a fragment's
-  // read then lie on distinct banks.
-  constexpr int kRowPieces = kUnits / 1024, kPieces = kRowPieces + kHead / 1024;
-  static_assert(kRowPieces % (4 * WAVES) == 0, "a wave's row pieces come in fours");
+  // a chunk's operands, straight from memory to LDS as they lie, 4 KiB a wave
+  // and turn (the last one 2)
+  constexpr int kRowQuads = kUnits / 4096, kQuads = kRowQuads + (kHead + 2048) / 4096;
+  static_assert(kUnits % 4096 == 0 && kHead % 4096 == 2048, "whole turns");
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds;
-  uint32_t row_off[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) row_off[i] = 1024 * i + 256 * grp + 16 * (col ^ (4 * i + grp));
   auto fetch = [&](int c) {
     const uint32_t to = lds0 + (uint32_t)((c % BUFS) * kBuf);
 #pragma unroll
-    for (int i = 0; i < kRowPieces / WAVES; ++i) {
-      const int x = (i & ~3) * WAVES + 4 * wave;
-      dma16_at(unit + x * 1024, row_off[i & 3], to + (x + (i & 3)) * 1024);
-    }
-#pragma unroll
-    for (int i = 0; i < (kHead / 1024 + WAVES - 1) / WAVES; ++i) {
+    for (int i = 0; i < (kQuads + WAVES - 1) / WAVES; ++i) {
       const int x = i * WAVES + wave;  // wave-uniform
-      if (x < kHead / 1024) dma16_at(head + x * 1024, 16 * lane, to + kUnits + x * 1024);
+      if (x < kRowQuads) dma_kib<4>(unit + x * 4096, to + x * 4096);
+      else if (x < kQuads - 1) dma_kib<4>(head + (x - kRowQuads) * 4096, to + x * 4096);
+      else if (x == kQuads - 1) dma_kib<2>(head + (x - kRowQuads) * 4096, to + x * 4096);
     }
     unit += a.H * unit_bytes(SPLIT), head += a.HV * head_bytes(SPLIT);
   };
@@ -601,20 +618,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const float* scal = (const float*)(tiles + tile_bytes(SPLIT));
     auto rows_of = [&](int plane, int tile, int step) {  // 16 tokens by 32 columns k
       Operand<SPLIT> o;
-      const uint8_t* p = b + (plane * C + 16 * tile + col) * RS + 8 * (grp & 1);
-      const int x = 16 * ((4 * step + (grp >> 1)) ^ col), y = x ^ 32;
-      const uint2 lo = *(const uint2*)(p + x), hi = *(const uint2*)(p + y);
-      o.hi = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-      if constexpr (SPLIT) {
-        const uint2 z = *(const uint2*)(p + C * RS + x), u = *(const uint2*)(p + C * RS + y);
-        o.lo = u32x4_t{z.x, z.y, u.x, u.y};
-      }
+      const uint8_t* p = b + (plane * C + 16 * tile + col) * RS + 16 * ((4 * step + grp) ^ col);
+      o.hi = *(const u32x4_t*)p;
+      if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + C * RS);
       return o;
     };
     auto turned = [&](int tile, int step) {  // 16 columns k of the keys by 32 tokens
       Operand<SPLIT> o;
       const int row = 4 * grp + (col >> 2);
-      const uint8_t* p = b + (32 * step + row) * RS + 16 * ((2 * tile + ((col & 3) >> 1)) ^ row) + 8 * (col & 1);
+      const uint8_t* p = b + 32 * step * RS + unit_at(row, 4 * tile + (col & 3));
       auto read = [](const uint8_t* q) { return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q)); };
       const uint2 x = read(p), y = read(p + 16 * RS);
       o.hi = u32x4_t{x.x, x.y, y.x, y.y};
@@ -635,8 +647,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const f32x4_t* beta4 = (const f32x4_t*)scal;
     const f32x4_t* grow4 = (const f32x4_t*)(scal + C);
     const f32x4_t* end4 = (const f32x4_t*)(scal + 2 * C);
+    const f32x4_t* held4 = (const f32x4_t*)(scal + 3 * C);
     const float total = scal[2 * C - 1];
-    const int bad_token = __builtin_amdgcn_readfirstlane(((const int*)scal)[3 * C]);
+    const int bad_token = __builtin_amdgcn_readfirstlane(((const int*)scal)[4 * C]);
 
     float v[NV][4][4];
 #pragma unroll
@@ -671,16 +684,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     GDNR_COMPILER_FENCE();
 
     // V-rows with a value that is not finite: zeros here, NaN from its token on
-    uint32_t ms[NV], mv[NV];
+    float bound[NV];  // |R| and |U| are at most 64 (|v| + 12 |S|)
     auto largest = [&](int nv) {
-      uint32_t x = 0, y = 0;
+      float x = 0.f, x2 = 0.f, y = 0.f;
 #pragma unroll
-      for (int kt = 0; kt < 8; ++kt)
+      for (int kt = 0; kt < 8; ++kt) x = max3_abs(x, S[nv][kt][0], S[nv][kt][1]), x2 = max3_abs(x2, S[nv][kt][2], S[nv][kt][3]);
+      x = __builtin_elementwise_maximum(x, x2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x = max(x, abs_bits(S[nv][kt][j]));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) y = max(y, abs_bits(v[nv][i >> 2][i & 3]));
-      ms[nv] = column_max(x), mv[nv] = column_max(y);
+      for (int i = 0; i < 16; i += 2) y = max3_abs(y, v[nv][i >> 2][i & 3], v[nv][i >> 2][(i & 3) + 1]);
+      bound[nv] = column_max(max3_abs(12.f * inv[nv] * x, y, 0.f));
     };
     int first[NV];
     bool any_bad = bad_token < C;
@@ -688,39 +700,53 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     for (int nv = 0; nv < NV; ++nv) {
       first[nv] = C;
       largest(nv);
-      any_bad |= __any(ms[nv] >= 0x7F800000u || mv[nv] >= 0x7F800000u);
+      any_bad |= __any(!finite(bound[nv]));
     }
     if (any_bad) {
 #pragma unroll
       for (int nv = 0; nv < NV; ++nv) {
-        uint32_t at = ms[nv] >= 0x7F800000u ? 0 : C;
+        float at = C;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float& x = v[nv][i >> 2][i & 3];
-          if (abs_bits(x) >= 0x7F800000u) at = min(at, (uint32_t)(16 * (i >> 2) + 4 * grp + (i & 3))), x = 0.f;
+          if (!finite(x)) at = fminf(at, (float)(16 * (i >> 2) + 4 * grp + (i & 3))), x = 0.f;
         }
 #pragma unroll
         for (int kt = 0; kt < 8; ++kt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (abs_bits(S[nv][kt][j]) >= 0x7F800000u) S[nv][kt][j] = 0.f;
-        first[nv] = min((int)(C - column_max(C - at)), bad_token);
+            if (!finite(S[nv][kt][j])) S[nv][kt][j] = 0.f, at = 0.f;
+        first[nv] = min(C - (int)column_max(C - at), bad_token);
         largest(nv);
       }
     }
-    // each row's power of two: |R| and |U| are at most 64 (|v| + 12 |S|)
-    Operand<SPLIT> bs[NV][4];
+    // Each row's power of two puts 64 times its bound between 2^9 and 2^15. It
+    // stays what it was while it does: then nothing is rescaled.
+    bool same = true;
+    float ratio[NV];
 #pragma unroll
     for (int nv = 0; nv < NV; ++nv) {
-      const float bound = fmaxf(__uint_as_float(mv[nv]), 12.f * __uint_as_float(ms[nv]) * inv[nv]);
-      const uint32_t ex = min(max((__float_as_uint(bound) >> 23) + 7, 15u), 254u);
-      const float s_new = __uint_as_float((268u - ex) << 23), ratio = fminf(s_new * inv[nv], 0x1p126f);
+      const uint32_t ex = min(max((__float_as_uint(bound[nv]) >> 23) + 7, 21u), 254u);
+      const float scaled = bound[nv] * sc[nv];
+      ratio[nv] = 1.f;
+      if (!(scaled < 0x1p8f && scaled >= 0x1p2f)) {
+        const float s_new = __uint_as_float((268u - ex) << 23);
+        ratio[nv] = fminf(s_new * inv[nv], 0x1p126f);
+        sc[nv] = s_new, inv[nv] = __uint_as_float((ex - 14u) << 23);
+      }
+      same &= ratio[nv] == 1.f;
+    }
+    if (!__all(same)) {
 #pragma unroll
-      for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= ratio;
-      sc[nv] = s_new, inv[nv] = __uint_as_float((ex - 14u) << 23);
+      for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+        for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= ratio[nv];
+    }
+    Operand<SPLIT> bs[NV][4];
+#pragma unroll
+    for (int nv = 0; nv < NV; ++nv)
 #pragma unroll
       for (int s = 0; s < 4; ++s) bs[nv][s] = operand<SPLIT>(S[nv][2 * s], S[nv][2 * s + 1]);
-    }
 
     // The products. Their LDS operands are read a stage or more before they
     // are used, which the fences keep the compiler from undoing: a read just
@@ -747,9 +773,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int s = 0; s <= tt / 2; ++s) tf[tri(tt, s)] = triangle(base, tt, s);
     };
-    f32x4_t be[4], gr[4];
+    f32x4_t be[4], bg[4];
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) be[tt] = beta4[4 * tt + grp], gr[tt] = grow4[4 * tt + grp];
+    for (int tt = 0; tt < 4; ++tt) be[tt] = beta4[4 * tt + grp], bg[tt] = held4[4 * tt + grp];
     if constexpr (!SPLIT) read_triangle(0);
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) read_rows(P, s);
@@ -761,7 +787,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
       for (int nv = 0; nv < NV; ++nv)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[nv][tt][j] = be[tt][j] * (v[nv][tt][j] * sc[nv] - gr[tt][j] * kDown * u[nv][tt][j]);
+        for (int j = 0; j < 4; ++j) u[nv][tt][j] = fmaf(bg[tt][j], u[nv][tt][j], be[tt][j] * (v[nv][tt][j] * sc[nv]));
 #pragma unroll
     for (int nv = 0; nv < NV; ++nv)
 #pragma unroll
@@ -831,6 +857,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     }
     // the outputs
     if constexpr (SPLIT) read_triangle(kTri);
+    f32x4_t gr[4];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) gr[tt] = grow4[4 * tt + grp];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -914,6 +943,10 @@ int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
 }
 template <class Act, class St, bool SPLIT>
 int launch_scan(const PrefillArgs& a, hipStream_t s) {
+  // all of a head's V-rows in one workgroup once that fills the card
+  const int64_t heads = (int64_t)a.N * a.HV;
+  if (a.V % 128 == 0 && heads * (a.V / 128) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 8, 1>(a, s);
+  if (a.V % 64 == 0 && heads * (a.V / 64) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 4, 1>(a, s);
   return launch_scan_as<Act, St, SPLIT, 2, 1>(a, s);
 }
 
