@@ -285,7 +285,7 @@ __device__ __forceinline__ float exp2_diff(double d) {
 // (rows i on a lane's registers, columns t on lanes), which is the order that
 // the scan's operands take them in.
 template <class Act, bool GATE_F32, bool SPLIT>
-__global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 : 4, SPLIT ? 2 : 4))) void chunk_prep_kernel(const PrefillArgs a) {
   using Gate = typename std::conditional<GATE_F32, ActF32, Act>::type;
   constexpr int ES = Act::kBytes, RS = 2 * K + 16, P = SPLIT ? 2 : 1;  // LDS row of a key or query, halves
   constexpr int kUnits = 2 * P * C * RS, MS = 68 * 4, kM = C * MS;      // [i][t] f32 of M, per head
@@ -311,19 +311,32 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
   if (len <= 0) return;
   const Work w = work_of(a, SPLIT);
   if (threadIdx.x == 0) bad_key = C;
-  __syncthreads();
 
-  // unit keys and queries, 16 lanes a row
+  // every row's keys and queries, 16 lanes a row, and the gates of the first
+  // two value heads are asked for at once
   uint8_t* unit = w.unit + ((int64_t)slot * a.H + h) * unit_bytes(SPLIT);
+  Raw<Act, 8> rows[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int t = min(16 * (i & 3) + 4 * wave + grp, len - 1);
+    rows[i].load((const uint8_t*)a.mixed + ((int64_t)(row0 + t) * a.mx_t + (i >= 4 ? h : a.H + h) * K + 8 * col) * ES);
+  }
+  float ga = 0.f, gb = 0.f, g_log = 0.f, g_bias = 0.f;
+  auto load_gates = [&](int g0) {
+    const int hv = h * a.G + min(g0 + wave, a.G - 1);
+    const int64_t at = row0 + min(lane, len - 1);
+    ga = Gate::ld(a.a, at * a.a_t + hv * a.a_h), gb = Gate::ld(a.bgate, at * a.bg_t + hv * a.bg_h);
+    g_log = a.a_log[hv * a.al_s], g_bias = a.dt_bias[hv * a.db_s];
+  };
+  load_gates(0);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const bool is_q = i >= 4;
     const int t = 16 * (i & 3) + 4 * wave + grp;
     float x[8], ss = 0.f;
-    Raw<Act, 8> r;
-    if (t < len) r.load((const uint8_t*)a.mixed + ((int64_t)(row0 + t) * a.mx_t + (is_q ? h : a.H + h) * K + 8 * col) * ES);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = t < len ? r[e] : 0.f, ss = fmaf(x[e], x[e], ss);
+    for (int e = 0; e < 8; ++e) x[e] = t < len ? rows[i][e] : 0.f, ss = fmaf(x[e], x[e], ss);
     ss = sum16(ss);
     float f = 1.f / sqrtf(ss + 1e-6f);
     if (!is_q && !(ss < __builtin_inff())) {
@@ -373,12 +386,12 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
     __syncthreads();  // the units (or the last heads' M) are no longer read
     if (wave < heads) {
       const int hv = h * a.G + g0 + wave, t = lane;
-      const int64_t at = row0 + t;
       float g = 0.f, beta = 0.f;
       bool bad = t >= bad_key;
+      if (g0) load_gates(g0);
       if (t < len) {
-        g = log_decay(Gate::ld(a.a, at * a.a_t + hv * a.a_h) + a.dt_bias[hv * a.db_s], a.a_log[hv * a.al_s]);
-        beta = sigmoid(Gate::ld(a.bgate, at * a.bg_t + hv * a.bg_h));
+        g = log_decay(ga + g_bias, g_log);
+        beta = sigmoid(gb);
         bad |= g != g || beta != beta || g > 3e38f;
       }
       const uint64_t bads = __ballot(bad && t < len);
@@ -435,17 +448,17 @@ __global__ __launch_bounds__(256) void chunk_prep_kernel(const PrefillArgs a) {
     // x (I + M) = e_t, the last column first. It takes M's place.
     if (grp < heads) {
       uint8_t* m = lds + grp * kM + 16 * wave * (MS + 4);
-      f32x4_t row[16][4];
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-#pragma unroll
-        for (int j = (i + 1) / 4; j < 4; ++j) row[i][j] = *(const f32x4_t*)(m + i * MS + 16 * j);
       float x[16];
 #pragma unroll
       for (int i = 15; i >= 0; --i) {
         x[i] = col == i ? 1.f : 0.f;
 #pragma unroll
-        for (int j = 15; j > i; --j) x[i] = fmaf(-x[j], row[i][j >> 2][j & 3], x[i]);
+        for (int q = 3; q >= (i + 1) / 4; --q) {
+          const f32x4_t row = *(const f32x4_t*)(m + i * MS + 16 * q);
+#pragma unroll
+          for (int j = 3; j >= 0; --j)
+            if (4 * q + j > i) x[i] = fmaf(-x[4 * q + j], row[j], x[i]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) *(float*)(m + i * MS + 4 * col) = x[i];
