@@ -1350,22 +1350,9 @@ int check_cache(const gdnr_tensor* c, const char* name, int act, int64_t heads, 
   return GDNR_OK;
 }
 
-// Keys a workgroup of the attention walks, and how many such pieces the
-// longest context has. A context is cut while the launch has fewer than four
-// workgroups a compute unit, into whole steps of its four waves (128 keys), at
-// least 256 keys: a shorter piece costs as much to join as to walk.
-void attention_pieces(int64_t T, int64_t N, int64_t HQ, int64_t HKV, int64_t max_context, int32_t* piece, int32_t* pieces) {
-  const int64_t G = HQ / HKV, gt = G < 16 ? G : 16, groups = (T / (16 / gt) + N) * HKV * ((G + 15) / 16);
-  const int64_t want = 4 * (int64_t)gdnr::device_cus();
-  int64_t p = max_context;
-  if (groups < want) p = (max_context * groups + want - 1) / want;
-  p = (p + 127) / 128 * 128;
-  if (p < 256) p = 256;
-  *piece = (int32_t)(p < INT32_MAX ? p : INT32_MAX);
-  *pieces = max_context ? (int32_t)((max_context + p - 1) / p) : 1;
-}
-int64_t attention_workspace(int64_t T, int64_t HQ, int64_t D, int32_t pieces) {
-  return pieces > 1 ? (int64_t)pieces * T * HQ * (D + 2) * 4 : 0;
+int64_t attention_workspace(const gdnr::AttentionArgs& a) {
+  const int64_t pieces = std::max(a.pieces[0], a.pieces[1]);
+  return pieces > 1 ? pieces * a.T * a.HQ * (a.D + 2) * 4 : 0;
 }
 }  // namespace
 
@@ -1515,9 +1502,15 @@ int64_t gdnr_paged_attention_workspace(int64_t tokens, int64_t sequences, int32_
     fail(GDNR_ERR_INVALID_ARGUMENT, "tokens, sequences and max_context must not be negative, heads a multiple of kv_heads");
     return -1;
   }
-  int32_t piece, pieces;
-  attention_pieces(tokens, sequences, heads, kv_heads, max_context, &piece, &pieces);
-  return attention_workspace(tokens, heads, head_dim, pieces);
+  if (tokens > kMaxTokens || sequences > kMaxSequences) {
+    fail(GDNR_ERR_UNSUPPORTED, "%lld tokens or %lld sequences are too many", (long long)tokens, (long long)sequences);
+    return -1;
+  }
+  gdnr::AttentionArgs a = {};
+  a.T = (int32_t)tokens, a.N = (int32_t)sequences, a.HQ = heads, a.HKV = kv_heads, a.G = heads / kv_heads, a.D = head_dim;
+  a.max_context = (int32_t)max_context;
+  gdnr::plan_attention(&a);
+  return attention_workspace(a);
 }
 
 int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const gdnr_tensor* v_cache,
@@ -1556,9 +1549,11 @@ int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const
   if (HQ > 4096) return fail(GDNR_ERR_UNSUPPORTED, "%lld heads exceed 4096", (long long)HQ);
   if (T * N == 0) return GDNR_OK;
   gdnr::AttentionArgs r = {};
-  attention_pieces(T, N, HQ, HKV, max_context, &r.piece, &r.pieces);
-  if (r.pieces > 65535) return fail(GDNR_ERR_UNSUPPORTED, "%d pieces of the context exceed 65535", r.pieces);
-  GDNR_TRY(check_workspace(workspace, attention_workspace(T, HQ, D, r.pieces)));
+  r.T = (int32_t)T, r.N = (int32_t)N, r.HQ = (int32_t)HQ, r.HKV = (int32_t)HKV, r.G = (int32_t)(HQ / HKV), r.D = (int32_t)D;
+  r.max_context = max_context;
+  gdnr::plan_attention(&r);
+  if (std::max(r.pieces[0], r.pieces[1]) > 65535) return fail(GDNR_ERR_UNSUPPORTED, "a context of %d keys has too many pieces", max_context);
+  GDNR_TRY(check_workspace(workspace, attention_workspace(r)));
   r.q = q->data, r.q_t = q->strides[0], r.q_h = q->strides[1];
   r.k_cache = k_cache->data, r.kc_p = k_cache->strides[0], r.kc_t = k_cache->strides[1], r.kc_h = k_cache->strides[2];
   r.v_cache = v_cache->data, r.vc_p = v_cache->strides[0], r.vc_t = v_cache->strides[1], r.vc_h = v_cache->strides[2];
@@ -1566,12 +1561,11 @@ int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const
   r.cu = (const int32_t*)cu_seqlens->data, r.cu_s = cu_seqlens->strides[0];
   r.context = (const int32_t*)context_lens->data, r.cx_s = context_lens->strides[0];
   r.out = out->data, r.o_t = out->strides[0], r.o_h = out->strides[1];
-  if (r.pieces > 1) {
+  if (const int64_t most = std::max(r.pieces[0], r.pieces[1]); most > 1) {
     r.part = (float*)workspace->data;
-    r.part_ml = r.part + (int64_t)r.pieces * T * HQ * D;
+    r.part_ml = r.part + most * T * HQ * D;
   }
-  r.T = (int32_t)T, r.N = (int32_t)N, r.HQ = (int32_t)HQ, r.HKV = (int32_t)HKV, r.G = (int32_t)(HQ / HKV), r.D = (int32_t)D;
-  r.page = (int32_t)page, r.n_pages = (int32_t)pages, r.max_context = max_context;
+  r.page = (int32_t)page, r.n_pages = (int32_t)pages;
   r.scale_log2 = scale * 1.4426950408889634f;
   return hip_status(gdnr::launch_attention(r, act, stream));
 }

@@ -6,13 +6,20 @@
 // keys of head h / G.
 //
 // One pass over the keys with a running maximum and sum (f32). The rows of a
-// workgroup are the (token, query head of the group) pairs of one key head, 16
-// to a tile, so the keys of a group are read once. Its four waves take 32 keys
-// each in turn and join at the end. The scores are formed transposed,
+// workgroup are the (token, query head of the group) pairs of one key head, so
+// the keys of a group are read once. The scores are formed transposed,
 // K (keys x D) by Q^T: a lane then holds 8 keys of one row, which is, as it
 // stands, the operand of V^T (D x keys) by P^T -- the contraction may take the
 // keys in any order as long as both operands do. V passes through LDS, where
 // the transposing read turns it.
+//
+// few_kernel: sequences of up to 16 rows (a decoded token of a group of up to
+// 16 heads). Bound by the cache's bytes: 16 rows a workgroup, whose four waves
+// take 32 keys each in turn, and long contexts in pieces.
+// tile_kernel: the others. Bound by the matrix products and the exponentials:
+// 128 rows a workgroup (64 at D = 256), 32 (16) a wave, all on the same keys.
+// A context is cut into pieces where the rows alone do not fill the card, and
+// join_kernel adds the pieces in their order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -30,7 +37,7 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 
 constexpr int kRows = 16;     // rows of a tile
-constexpr int kKeys = 32;     // keys of a wave's step
+constexpr int kKeys = 32;     // few_kernel: keys of a wave's step
 constexpr int kWaves = 4;
 
 template <class Act>
@@ -62,12 +69,50 @@ __device__ __forceinline__ bool nonfinite8(u32x4_t w) {
 }
 // over the lanes of one column (lane & 15), in each of them
 __device__ __forceinline__ float column_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  const uint32_t b = __float_as_uint(x);
+  const auto half = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t h = __float_as_uint(fmaxf(__uint_as_float(half[0]), __uint_as_float(half[1])));
+  const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+  return fmaxf(__uint_as_float(row[0]), __uint_as_float(row[1]));
 }
 __device__ __forceinline__ float column_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  const uint32_t b = __float_as_uint(x);
+  const auto half = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t h = __float_as_uint(__uint_as_float(half[0]) + __uint_as_float(half[1]));
+  const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+  return __uint_as_float(row[0]) + __uint_as_float(row[1]);
+}
+// x *= f and x += a b in the registers where x lies: of the two sides of a
+// branch, the one that leaves x alone then has nothing to copy
+__device__ __forceinline__ void scale_in_place(f32x4_t& x, float f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y = x[i];
+    asm volatile("v_mul_f32 %0, %1, %0" : "+v"(y) : "v"(f));
+    x[i] = y;
+  }
+}
+__device__ __forceinline__ void shift_in_place(f32x4_t& x, float d) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y = x[i];
+    asm volatile("v_add_f32 %0, %1, %0" : "+v"(y) : "v"(d));
+    x[i] = y;
+  }
+}
+__device__ __forceinline__ void add_in_place(f32x4_t& x, float a, f32x4_t b) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y = x[i];
+    asm volatile("v_fmac_f32 %0, %1, %2" : "+v"(y) : "v"(a), "v"(b[i]));
+    x[i] = y;
+  }
+}
+// page and offset of a key (1 / page is off by a rounding: by at most one page)
+__device__ __forceinline__ void page_of(int key, int page, double inv_page, int& p, int& r) {
+  p = (int)((double)key * inv_page), r = key - p * page;
+  if (r < 0) --p, r += page;
+  if (r >= page) ++p, r -= page;
 }
 
 // Number of sequences n < N with cu[n] / per + n * every <= x (cu clamped to
@@ -95,6 +140,10 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int n) {
   s.context = min(max(__builtin_amdgcn_readfirstlane(a.context[n * a.cx_s]), 0), a.max_context);
   return s;
 }
+// whether few_kernel takes the sequence (tile_kernel otherwise)
+__device__ __forceinline__ bool few_rows(const AttentionArgs& a, const Span& s) {
+  return (int64_t)(s.end - s.begin) * min(a.G, kRows) <= a.few_rows;
+}
 // keys that token t of the sequence sees
 __device__ __forceinline__ int visible(const Span& s, int t) { return min(max(s.context - s.end + t + 1, 0), s.context); }
 
@@ -109,22 +158,23 @@ constexpr int lds_bytes() {
 }
 
 template <class Act, int D>
-__global__ __launch_bounds__(256) void attention_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(256) void few_kernel(const AttentionArgs a) {
   constexpr int KSTEPS = D / 32, DT = D / 16, LPR = D / 8, KPI = 64 / LPR, NV = kKeys / KPI;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int gt = min(a.G, kRows), tb = kRows / gt;  // heads and tokens of a tile
-  const int n = sequences_up_to(a, blockIdx.x, tb, 1) - 1;
+  const int n = sequences_up_to(a, blockIdx.y, tb, 1) - 1;
   if (n < 0) return;
   const Span sq = span_of(a, n);
-  const int tok0 = sq.begin + ((int)blockIdx.x - sq.begin / tb - n) * tb;
-  if (tok0 >= sq.end) return;
+  const int tok0 = sq.begin + ((int)blockIdx.y - sq.begin / tb - n) * tb;
+  if (tok0 >= sq.end || !few_rows(a, sq)) return;
   const int head_tiles = (a.G + kRows - 1) / kRows;
-  const int hk = blockIdx.y / head_tiles, ht = blockIdx.y - hk * head_tiles;
+  const int hk = blockIdx.x / head_tiles, ht = blockIdx.x - hk * head_tiles;
   const int last = min(tok0 + tb, sq.end) - 1;
-  const int k_begin = (int)blockIdx.z * a.piece, k_end = min(visible(sq, last), k_begin + a.piece);
-  if (k_begin >= k_end && (a.pieces > 1 || blockIdx.z > 0)) return;
+  const int piece = a.piece[0], pieces = a.pieces[0];
+  const int k_begin = (int)blockIdx.z * piece, k_end = min(visible(sq, last), k_begin + piece);
+  if (k_begin >= k_end && (pieces > 1 || blockIdx.z > 0)) return;
 
   // this lane's row
   const int rt = tok0 + col / gt, rh = ht * kRows + col % gt;
@@ -148,9 +198,8 @@ __global__ __launch_bounds__(256) void attention_kernel(const AttentionArgs a) {
   uint32_t k_row, v_row;
   auto find_rows = [&](int key0) {
     const int key = min(key0 + (lane & 31), k_end - 1);
-    int p = (int)((double)key * inv_page), r = key - p * a.page;
-    if (r < 0) --p, r += a.page;
-    if (r >= a.page) ++p, r -= a.page;
+    int p, r;
+    page_of(key, a.page, inv_page, p, r);
     const int at = min(max(table[p], 0), a.n_pages - 1);
     k_row = (uint32_t)((at * a.kc_p + r * a.kc_t) >> 3);
     v_row = (uint32_t)((at * a.vc_p + r * a.vc_t) >> 3);
@@ -211,7 +260,7 @@ __global__ __launch_bounds__(256) void attention_kernel(const AttentionArgs a) {
       const float f = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
       l_run *= f;
 #pragma unroll
-      for (int i = 0; i < DT; ++i) o[i] *= f;
+      for (int i = 0; i < DT; ++i) scale_in_place(o[i], f);
       m_run = m_new;
     }
     const float base = m_run == -__builtin_inff() ? 0.f : m_run;
@@ -221,21 +270,21 @@ __global__ __launch_bounds__(256) void attention_kernel(const AttentionArgs a) {
     if (__any(bad)) {
       // a value that some rows must not see is infinite or NaN, and a product
       // with its weight 0 would show it to them: this step key by key
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
 #pragma nounroll
-        for (int g = 0; g < 4; ++g) {
-          const int key = 16 * (e >> 2) + 4 * g + (e & 3);
-          const float pk = __shfl(p[e], col + 16 * g);
-          const bool seen = key0 + key < min(vis, k_end);
+      for (int key = 0; key < kKeys; ++key) {
+        float pk = 0.f;
 #pragma unroll
-          for (int i = 0; i < DT; ++i) {
-            const uint2 w = *(const uint2*)(vt + key * v_stride<D>() + 32 * i + 8 * grp);
-            const float2 lo = Act::from_pair(w.x), hi = Act::from_pair(w.y);
-            const f32x4_t v = {lo.x, lo.y, hi.x, hi.y};
-            if (seen) o[i] += pk * v;
-          }
+        for (int e = 0; e < 8; ++e)
+          if (4 * (key >> 4) + (key & 3) == e) pk = p[e];
+        pk = __shfl(pk, col + 16 * ((key >> 2) & 3));
+        const uint32_t seen = key0 + key < min(vis, k_end) ? ~0u : 0u;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const uint2 w = *(const uint2*)(vt + key * v_stride<D>() + 32 * i + 8 * grp);
+          const float2 lo = Act::from_pair(w.x & seen), hi = Act::from_pair(w.y & seen);
+          add_in_place(o[i], pk, f32x4_t{lo.x, lo.y, hi.x, hi.y});
         }
+      }
       continue;
     }
     // (the sum is of the unrounded weights; rounding them to the cache's type
@@ -270,7 +319,7 @@ __global__ __launch_bounds__(256) void attention_kernel(const AttentionArgs a) {
     l += f[w] * ml[2 * (w * kRows + row) + 1];
   }
   const int qh = hk * a.G + head;
-  const float norm = a.pieces > 1 ? 1.f : visible(sq, t) == 0 ? 0.f : 1.f / l;
+  const float norm = pieces > 1 ? 1.f : visible(sq, t) == 0 ? 0.f : 1.f / l;
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) {
     const int d = 64 * i + 4 * dl;
@@ -278,15 +327,310 @@ __global__ __launch_bounds__(256) void attention_kernel(const AttentionArgs a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += f[w] * *(const f32x4_t*)(lds + (w * kRows + row) * o_stride<D>() + 4 * d);
     sum *= norm;
-    if (a.pieces > 1) {
+    if (pieces > 1) {
       *(f32x4_t*)(a.part + (((int64_t)blockIdx.z * a.T + t) * a.HQ + qh) * D + d) = sum;
     } else {
       *(uint2*)((uint8_t*)a.out + (t * a.o_t + qh * a.o_h + d) * 2) = make_uint2(pack2<Act>(sum[0], sum[1]), pack2<Act>(sum[2], sum[3]));
     }
   }
-  if (a.pieces > 1 && dl == 0) {
+  if (pieces > 1 && dl == 0) {
     float* p = a.part_ml + (((int64_t)blockIdx.z * a.T + t) * a.HQ + qh) * 2;
     p[0] = top, p[1] = l;
+  }
+}
+
+// 16-byte piece p of row r of a tile of D-element rows in LDS lies at p ^ key:
+// 16 rows' pieces then fall on distinct banks (rows of 128 bytes lie two to a
+// bank window)
+template <int D>
+__device__ __forceinline__ int row_key(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+
+template <int D>
+struct Tile {
+  static constexpr int NT = D == 256 ? 1 : 2;      // 16-row tiles a wave
+  static constexpr int ROWS = kWaves * NT * 16;    // rows a workgroup
+  static constexpr int KEYS = D == 256 ? 32 : 64;  // keys a step
+  static constexpr int KB = KEYS * 2 * D;          // bytes of a step's keys (and of its values)
+  static constexpr int LDS = 4 * KB;               // two steps' keys and values
+};
+
+// 128 rows against the same keys. A step's keys and values go from the cache
+// straight to LDS while the step before is computed. A wave keeps its rows'
+// queries, scores and outputs in registers; the keys' fragment it reads from
+// LDS serves both of its row tiles.
+template <class Act, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(const AttentionArgs a) {
+  using TL = Tile<D>;
+  constexpr int KSTEPS = D / 32, DT = D / 16, NT = TL::NT, KEYS = TL::KEYS, MT = KEYS / 16, PPR = D / 8;
+  constexpr int RPI = 64 / PPR;                     // rows of an LDS copy
+  constexpr int COPIES = KEYS / RPI / kWaves;       // copies of keys (and of values) a wave and step
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int gt = min(a.G, TL::ROWS), tb = TL::ROWS / gt;  // heads and tokens of a workgroup
+  const int n = sequences_up_to(a, blockIdx.y, tb, 1) - 1;
+  if (n < 0) return;
+  const Span sq = span_of(a, n);
+  const int tok0 = sq.begin + ((int)blockIdx.y - sq.begin / tb - n) * tb;
+  if (tok0 >= sq.end || few_rows(a, sq)) return;
+  const int head_tiles = (a.G + TL::ROWS - 1) / TL::ROWS;
+  const int hk = blockIdx.x / head_tiles, ht = blockIdx.x - hk * head_tiles;
+  const int last = min(tok0 + tb, sq.end) - 1;
+  const int piece = a.piece[1], pieces = a.pieces[1];
+  const int k_begin = (int)blockIdx.z * piece, k_end = min(visible(sq, last), k_begin + piece);
+  if (k_begin >= k_end && (pieces > 1 || blockIdx.z > 0)) return;
+
+  // this lane's rows
+  int rt[NT], rh[NT], vis[NT];
+  bool live[NT];
+  u32x4_t q[NT][KSTEPS];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = (wave * NT + nt) * 16 + col;
+    rt[nt] = tok0 + r / gt, rh[nt] = ht * TL::ROWS + r % gt;
+    live[nt] = r / gt < tb && rt[nt] < sq.end && rh[nt] < a.G;
+    vis[nt] = live[nt] ? min(visible(sq, rt[nt]), k_end) : 0;
+    const uint8_t* qp = (const uint8_t*)a.q + (rt[nt] * a.q_t + (hk * a.G + rh[nt]) * a.q_h) * 2 + 16 * grp;
+#pragma unroll
+    for (int i = 0; i < KSTEPS; ++i) q[nt][i] = live[nt] ? *(const u32x4_t*)(qp + 64 * i) : u32x4_t{0, 0, 0, 0};
+  }
+  const int vis_all = min(visible(sq, tok0), k_end);  // every live row sees these
+  // scores grow with the products: a negative scale turns the queries' signs
+  if (a.scale_log2 < 0.f) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < KSTEPS; ++i) q[nt][i] ^= 0x80008000u;
+  }
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);  // (a masked -inf stays one)
+
+  // copies: wave w's rows of a step are those of copies w, w + 4, ...; lane l
+  // finds row l of them, in 16-byte units from the caches' bases
+  constexpr int OWN = COPIES * RPI;
+  const double inv_page = 1.0 / a.page;
+  const int32_t* table = a.table + n * a.tb_n;
+  const uint8_t* kbase = (const uint8_t*)a.k_cache + hk * a.kc_h * 2;
+  const uint8_t* vbase = (const uint8_t*)a.v_cache + hk * a.vc_h * 2;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds + wave * 1024;
+  const uint32_t k_page = (uint32_t)(a.kc_p >> 3), k_tok = (uint32_t)(a.kc_t >> 3);
+  const uint32_t v_page = (uint32_t)(a.vc_p >> 3), v_tok = (uint32_t)(a.vc_t >> 3);
+  const int own = lane % OWN, own_row = ((own / RPI) * kWaves + wave) * RPI + own % RPI;
+  int pg, off;
+  auto find_rows = [&](int key0) {
+    int p;
+    page_of(min(key0 + own_row, k_end - 1), a.page, inv_page, p, off);
+    pg = table[p];
+  };
+  auto copy = [&](int buf) {
+    const uint32_t at = min(max(pg, 0), a.n_pages - 1);
+    const uint32_t k_row = at * k_page + off * k_tok, v_row = at * v_page + off * v_tok;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int from = i * RPI + lane / PPR, piece16 = (lane % PPR) ^ row_key<D>((i * kWaves + wave) * RPI + lane / PPR);
+      const uint32_t to = lds0 + buf * 2 * TL::KB + i * kWaves * 1024;
+      dma16(kbase + (uint64_t)((uint32_t)__shfl((int)k_row, from) + (uint64_t)piece16) * 16, to);
+      dma16(vbase + (uint64_t)((uint32_t)__shfl((int)v_row, from) + (uint64_t)piece16) * 16, to + TL::KB);
+    }
+  };
+
+  f32x4_t o[NT][DT];
+  float m_run[NT], l_run[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m_run[nt] = -__builtin_inff(), l_run[nt] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[nt][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  if (k_begin < k_end) {
+    find_rows(k_begin);
+    copy(0);
+    if (k_begin + KEYS < k_end) find_rows(k_begin + KEYS);
+  }
+  int buf = 0, key0 = k_begin;
+  // one step; MASKED: some of its keys are not seen by every row
+  auto step = [&](auto tag) {
+    constexpr bool MASKED = decltype(tag)::value;
+    GDNR_WAIT_VMCNT(0);
+    __syncthreads();  // the step's keys and values are in LDS; the other buffer is no longer read
+    if (key0 + KEYS < k_end) {
+      copy(buf ^ 1);
+      if (key0 + 2 * KEYS < k_end) find_rows(key0 + 2 * KEYS);
+    }
+    const uint8_t* kt = lds + buf * 2 * TL::KB;
+    const uint8_t* vt = kt + TL::KB;
+    // (the fragments' addresses are formed where they are used: kept across
+    // steps they would take the registers of the operands)
+    uint32_t k_key = row_key<D>(col) ^ grp, v_key = row_key<D>(4 * grp + (col >> 2)) ^ ((col & 3) >> 1);
+    asm volatile("" : "+v"(k_key), "+v"(v_key));
+    const uint8_t* kl = kt + col * 2 * D;
+    const uint8_t* vl = vt + (4 * grp + (col >> 2)) * 2 * D + 8 * (col & 1);
+
+    // S^T = K Q^T, two key tiles at a time
+    f32x4_t s[MT][NT];
+    u32x4_t kf[2][2][2];
+    constexpr int KH = 2, STAGES = MT / 2 * (KSTEPS / KH);
+    auto read_keys = [&](int st) {  // stage: key tiles 2 m2, 2 m2 + 1, k-steps KH h ..
+      const int m2 = st / (KSTEPS / KH), h = st % (KSTEPS / KH);
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < KH; ++i) {
+          kf[st & 1][m][i] = *(const u32x4_t*)(kl + 16 * (2 * m2 + m) * 2 * D + 16 * ((4 * (KH * h + i)) ^ k_key));
+        }
+    };
+    read_keys(0);
+#pragma unroll
+    for (int st = 0; st < STAGES; ++st) {
+      if (st + 1 < STAGES) read_keys(st + 1);
+      GDNR_COMPILER_FENCE();
+      const int m2 = st / (KSTEPS / KH), h = st % (KSTEPS / KH);
+#pragma unroll
+      for (int i = 0; i < KH; ++i)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            s[2 * m2 + m][nt] = mfma<Act>(kf[st & 1][m][i], q[nt][KH * h + i],
+                                          i + h == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : s[2 * m2 + m][nt]);
+    }
+    GDNR_COMPILER_FENCE();
+    // the values' fragments of 32 keys, read before the weights are formed
+    u32x4_t vf[DT];
+    auto read_values = [&](int half) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        const uint8_t* p = vl + 32 * half * 2 * D + 16 * ((2 * i) ^ v_key);
+        const uint2 lo = transposed4(p), hi = transposed4(p + 32 * D);
+        vf[i] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+      }
+    };
+    read_values(0);
+    GDNR_COMPILER_FENCE();
+
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (key0 + 16 * m + 4 * grp + j >= vis[nt]) s[m][nt][j] = -__builtin_inff();
+    }
+    // The maximum follows the scores only when it falls 2^8 behind them: a
+    // weight then grows to 256 at most, and the outputs are rarely rescaled.
+    float top[NT];
+    bool behind = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      top[nt] = s[0][nt][0];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top[nt] = fmaxf(top[nt], s[m][nt][j]);
+      top[nt] = column_max(top[nt]);
+      behind |= top[nt] * scale > m_run[nt] + 8.f;
+    }
+    if (__any(behind)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float m_new = fmaxf(m_run[nt], top[nt] * scale);
+        const float f = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m_run[nt] - m_new);
+        l_run[nt] *= f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) scale_in_place(o[nt][i], f);
+        m_run[nt] = m_new;
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float base = m_run[nt] == -__builtin_inff() ? 0.f : -m_run[nt], f = scale;
+      if (__any(fabsf(base) > 0x1p24f)) {
+        // (a rounding of such a product may pass the exponent's range: both
+        // sides of the difference are rounded alike)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) scale_in_place(s[m][nt], f), shift_in_place(s[m][nt], base);
+        base = 0.f, f = 1.f;
+      }
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[m][nt][j] = __builtin_amdgcn_exp2f(fmaf(s[m][nt][j], f, base));
+          sum[j & 1] += s[m][nt][j];
+        }
+      l_run[nt] += sum[0] + sum[1];
+    }
+    if constexpr (MASKED) {
+      bool bad = false;
+#pragma nounroll
+      for (int i = lane; i < KEYS * PPR; i += 64) bad |= nonfinite8<Act>(*(const u32x4_t*)(vt + 16 * i));
+      if (__any(bad)) {
+        // a value that some rows must not see is infinite or NaN, and a product
+        // with its weight 0 would show it to them: this step key by key
+#pragma nounroll
+        for (int key = 0; key < KEYS; ++key)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float pk = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4 * MT; ++e)
+              if (4 * (key >> 4) + (key & 3) == e) pk = s[e >> 2][nt][e & 3];
+            pk = __shfl(pk, col + 16 * ((key >> 2) & 3));
+            const uint32_t seen = key0 + key < vis[nt] ? ~0u : 0u;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+              const uint2 w = *(const uint2*)(vt + key * 2 * D + 16 * ((2 * i + (grp >> 1)) ^ row_key<D>(key)) + 8 * (grp & 1));
+              const float2 lo = Act::from_pair(w.x & seen), hi = Act::from_pair(w.y & seen);
+              add_in_place(o[nt][i], pk, f32x4_t{lo.x, lo.y, hi.x, hi.y});
+            }
+          }
+        return;
+      }
+    }
+    // O^T += V^T P^T. (The sum is of the unrounded weights; rounding them to
+    // the cache's type costs the output about its own rounding.)
+#pragma unroll
+    for (int half = 0; half < MT / 2; ++half) {
+      u32x4_t pf[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const f32x4_t x = s[2 * half][nt], y = s[2 * half + 1][nt];
+        pf[nt] = u32x4_t{pack2<Act>(x[0], x[1]), pack2<Act>(x[2], x[3]), pack2<Act>(y[0], y[1]), pack2<Act>(y[2], y[3])};
+      }
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[nt][i] = mfma<Act>(vf[i], pf[nt], o[nt][i]);
+      if (half + 1 < MT / 2) {
+        GDNR_COMPILER_FENCE();
+        read_values(half + 1);
+        GDNR_COMPILER_FENCE();
+      }
+    }
+  };
+  for (; key0 + KEYS <= vis_all; key0 += KEYS, buf ^= 1) step(std::false_type{});
+  for (; key0 < k_end; key0 += KEYS, buf ^= 1) step(std::true_type{});
+
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float l = column_sum(l_run[nt]);
+    if (!live[nt]) continue;
+    const int qh = hk * a.G + rh[nt];
+    if (pieces > 1) {
+      const int64_t at = ((int64_t)blockIdx.z * a.T + rt[nt]) * a.HQ + qh;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) *(f32x4_t*)(a.part + at * D + 16 * i + 4 * grp) = o[nt][i];
+      if (grp == 0) a.part_ml[2 * at] = m_run[nt], a.part_ml[2 * at + 1] = l;
+    } else {
+      const float norm = vis[nt] == 0 ? 0.f : 1.f / l;
+      uint8_t* p = (uint8_t*)a.out + (rt[nt] * a.o_t + qh * a.o_h + 4 * grp) * 2;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        const f32x4_t x = o[nt][i] * norm;
+        *(uint2*)(p + 32 * i) = make_uint2(pack2<Act>(x[0], x[1]), pack2<Act>(x[2], x[3]));
+      }
+    }
   }
 }
 
@@ -300,8 +644,9 @@ __global__ __launch_bounds__(256) void join_kernel(const AttentionArgs a) {
   const int n = sequences_up_to(a, t, 1, 0) - 1;
   if (n < 0) return;
   const Span sq = span_of(a, n);
-  if (t >= sq.end) return;
-  const int vis = visible(sq, t), pieces = (vis + a.piece - 1) / a.piece;
+  const int kind = few_rows(a, sq) ? 0 : 1, piece = a.piece[kind];
+  if (t >= sq.end || a.pieces[kind] == 1) return;
+  const int vis = visible(sq, t), pieces = (vis + piece - 1) / piece;
   constexpr int E = D / 64;
   float acc[E] = {}, top = -__builtin_inff(), l = 0.f;
   for (int z = 0; z < pieces; ++z) {
@@ -327,14 +672,27 @@ __global__ __launch_bounds__(256) void join_kernel(const AttentionArgs a) {
 
 template <class Act, int D>
 int launch_dim(const AttentionArgs& a, hipStream_t s) {
-  const int gt = a.G < kRows ? a.G : kRows, tb = kRows / gt, head_tiles = (a.G + kRows - 1) / kRows;
-  if (lds_bytes<D>() > 64 * 1024) {  // (enabled per kernel and device; idempotent, cheap)
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_kernel<Act, D>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes<D>());
-    if (e != hipSuccess) return (int)e;
+  const auto grid = [&](int rows, int pieces) {  // key heads first: a head's workgroups share an XCD
+    const int gt = a.G < rows ? a.G : rows, tb = rows / gt;
+    return dim3(a.HKV * ((a.G + rows - 1) / rows), a.T / tb + a.N, pieces);
+  };
+  const auto launch = [&](auto kernel, int rows, int pieces, int lds) {
+    if (lds > 64 * 1024) {  // (enabled per kernel and device; idempotent, cheap)
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e != hipSuccess) return (int)e;
+    }
+    hipLaunchKernelGGL(kernel, grid(rows, pieces), dim3(256), lds, s, a);
+    return (int)hipGetLastError();
+  };
+  if (a.pieces[0]) {
+    const int rc = launch(few_kernel<Act, D>, kRows, a.pieces[0], lds_bytes<D>());
+    if (rc) return rc;
   }
-  hipLaunchKernelGGL((attention_kernel<Act, D>), dim3(a.T / tb + a.N, a.HKV * head_tiles, a.pieces), dim3(256), lds_bytes<D>(), s, a);
-  if (a.pieces > 1)
+  if (a.pieces[1]) {
+    const int rc = launch(tile_kernel<Act, D>, Tile<D>::ROWS, a.pieces[1], Tile<D>::LDS);
+    if (rc) return rc;
+  }
+  if (a.pieces[0] > 1 || a.pieces[1] > 1)
     hipLaunchKernelGGL((join_kernel<Act, D>), dim3((uint32_t)(((int64_t)a.T * a.HQ + 3) / 4)), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
@@ -346,6 +704,32 @@ int launch_act(const AttentionArgs& a, hipStream_t s) {
 }
 
 }  // namespace
+
+// Which kernels run (pieces 0: not that one), and the keys of a workgroup's
+// piece. The lengths are on the device; the host knows their number and sum.
+// Where a sequence has 16 rows or fewer on average, few_kernel takes all of
+// them; a single longer one is tile_kernel's; otherwise each takes its kind. A
+// context is cut while a kernel would have fewer than four (few) or two (tile)
+// workgroups a compute unit, into whole steps of 128 keys, at least 256: a
+// shorter piece costs as much to join as to walk.
+void plan_attention(AttentionArgs* a) {
+  const int64_t cus = device_cus(), rows = (int64_t)a->T * (a->G < kRows ? a->G : kRows);
+  const bool all_few = rows <= (int64_t)kRows * a->N, all_tile = !all_few && a->N == 1;
+  a->few_rows = all_few ? INT32_MAX : all_tile ? 0 : kRows;
+  const auto plan = [&](int kind, int tile_rows, int64_t want) {
+    const int64_t gt = a->G < tile_rows ? a->G : tile_rows, tb = tile_rows / gt;
+    const int64_t groups = (a->T / tb + a->N) * a->HKV * ((a->G + tile_rows - 1) / tile_rows);
+    int64_t p = a->max_context;
+    if (groups < want) p = (a->max_context * groups + want - 1) / want;
+    p = (p + 127) / 128 * 128;
+    if (p < 256) p = 256;
+    a->piece[kind] = (int32_t)(p < INT32_MAX ? p : INT32_MAX);
+    a->pieces[kind] = a->max_context ? (int32_t)((a->max_context + p - 1) / p) : 1;
+  };
+  a->pieces[0] = a->pieces[1] = 0;
+  if (!all_tile) plan(0, kRows, 4 * cus);
+  if (!all_few) plan(1, a->D == 256 ? 64 : 128, 2 * cus);
+}
 
 int launch_attention(const AttentionArgs& a, int act_dt, void* stream) {
   return act_dt == DT_BF16 ? launch_act<ActBF16>(a, (hipStream_t)stream) : launch_act<ActF16>(a, (hipStream_t)stream);

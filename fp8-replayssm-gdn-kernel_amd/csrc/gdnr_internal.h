@@ -216,7 +216,9 @@ struct AttentionArgs {
   float* part;       // [pieces, T, HQ, D] sums of p v, unnormalised
   float* part_ml;    // [pieces, T, HQ, 2] running maximum and sum
   int32_t T, N, HQ, HKV, G, D, page, n_pages, max_context;
-  int32_t piece, pieces;  // keys a workgroup walks, and the most pieces a context has
+  // keys a workgroup walks and the most such pieces a context has, for the
+  // sequences of few rows ([0], at most few_rows rows a key head) and the others ([1])
+  int32_t piece[2], pieces[2], few_rows;
   float scale_log2;       // scale * log2(e)
 };
 
@@ -265,6 +267,7 @@ int launch_rmw_packed(const RmwArgs& a, int state_dt, int act_dt, bool gate_f32,
 int64_t prefill_work_bytes(int64_t T, int64_t N, int32_t H, int32_t HV, int act_dt, int state_dt);
 int launch_prefill(const PrefillArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream);
 int launch_append(const AppendArgs& a, int act_dt, void* stream);
+void plan_attention(AttentionArgs* a);
 int launch_attention(const AttentionArgs& a, int act_dt, void* stream);
 int launch_format_quantize(const FormatArgs& a, void* stream);
 int launch_format_dequantize(const FormatArgs& a, void* stream);
