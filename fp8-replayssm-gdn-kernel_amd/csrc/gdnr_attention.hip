@@ -147,27 +147,38 @@ __device__ __forceinline__ bool few_rows(const AttentionArgs& a, const Span& s) 
 // keys that token t of the sequence sees
 __device__ __forceinline__ int visible(const Span& s, int t) { return min(max(s.context - s.end + t + 1, 0), s.context); }
 
+// 16-byte piece p of row r of a tile of D-element rows in LDS lies at p ^ key:
+// 16 rows' pieces then fall on distinct banks (rows of 128 bytes lie two to a
+// bank window)
 template <int D>
-constexpr int v_stride() { return 2 * D + 32; }  // bytes between V rows in LDS: 16 rows' 32-byte pieces on distinct banks
+__device__ __forceinline__ int row_key(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+
 template <int D>
 constexpr int o_stride() { return 4 * D + 16; }
 template <int D>
 constexpr int lds_bytes() {
-  const int v = kWaves * kKeys * v_stride<D>(), o = kWaves * kRows * o_stride<D>();
+  const int v = kWaves * kKeys * 2 * D, o = kWaves * kRows * o_stride<D>();
   return (v > o ? v : o) + kWaves * kRows * 8;
 }
 
+// A wave's step: its keys' scores from registers (a lane holds whole pieces of
+// two keys' rows, as the product takes them), its values from its part of the
+// LDS. The next step's keys are asked for once the scores have used this one's,
+// its values once the outputs have; two to four workgroups a compute unit
+// cover the waits.
 template <class Act, int D>
-__global__ __launch_bounds__(256) void few_kernel(const AttentionArgs a) {
-  constexpr int KSTEPS = D / 32, DT = D / 16, LPR = D / 8, KPI = 64 / LPR, NV = kKeys / KPI;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 ? 4 : 2))) void few_kernel(const AttentionArgs a) {
+  constexpr int KSTEPS = D / 32, DT = D / 16, PPR = D / 8, RPI = 64 / PPR, NV = kKeys / RPI;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int gt = min(a.G, kRows), tb = kRows / gt;  // heads and tokens of a tile
-  const int n = sequences_up_to(a, blockIdx.y, tb, 1) - 1;
+  // beside tile_kernel, one tile holds all rows of each sequence that is taken here
+  int n = blockIdx.y;
+  if (a.few_rows > kRows) n = sequences_up_to(a, n, tb, 1) - 1;
   if (n < 0) return;
   const Span sq = span_of(a, n);
-  const int tok0 = sq.begin + ((int)blockIdx.y - sq.begin / tb - n) * tb;
+  const int tok0 = a.few_rows > kRows ? sq.begin + ((int)blockIdx.y - sq.begin / tb - n) * tb : sq.begin;
   if (tok0 >= sq.end || !few_rows(a, sq)) return;
   const int head_tiles = (a.G + kRows - 1) / kRows;
   const int hk = blockIdx.x / head_tiles, ht = blockIdx.x - hk * head_tiles;
@@ -179,8 +190,8 @@ __global__ __launch_bounds__(256) void few_kernel(const AttentionArgs a) {
   // this lane's row
   const int rt = tok0 + col / gt, rh = ht * kRows + col % gt;
   const bool live = col / gt < tb && rt < sq.end && rh < a.G;
-  const int vis = live ? visible(sq, rt) : 0;
-  const int vis_all = visible(sq, tok0);  // every live row sees these
+  const int vis = live ? min(visible(sq, rt), k_end) : 0;
+  const int vis_all = min(visible(sq, tok0), k_end);  // every live row sees these
   u32x4_t q[KSTEPS];
   {
     const uint8_t* qp = (const uint8_t*)a.q + (rt * a.q_t + (hk * a.G + rh) * a.q_h) * 2 + 16 * grp;
@@ -188,39 +199,39 @@ __global__ __launch_bounds__(256) void few_kernel(const AttentionArgs a) {
     for (int i = 0; i < KSTEPS; ++i) q[i] = live ? *(const u32x4_t*)(qp + 64 * i) : u32x4_t{0, 0, 0, 0};
   }
 
-  uint8_t* vt = lds + wave * kKeys * v_stride<D>();
+  uint8_t* vt = lds + wave * kKeys * 2 * D;
+  const uint32_t vt_lds = (uint32_t)(uintptr_t)(lds_void_t*)vt;
   const double inv_page = 1.0 / a.page;
   const int32_t* table = a.table + n * a.tb_n;
   const uint8_t* kbase = (const uint8_t*)a.k_cache + hk * a.kc_h * 2 + 16 * grp;
-  const uint8_t* vbase = (const uint8_t*)a.v_cache + hk * a.vc_h * 2 + 16 * (lane % LPR);
+  const uint8_t* vbase = (const uint8_t*)a.v_cache + hk * a.vc_h * 2;
+  const uint32_t k_page = (uint32_t)(a.kc_p >> 3), k_tok = (uint32_t)(a.kc_t >> 3);
+  const uint32_t v_page = (uint32_t)(a.vc_p >> 3), v_tok = (uint32_t)(a.vc_t >> 3);
   // rows of a step's keys, in 16-byte units from the caches' bases: lane l
-  // finds key l & 31's
-  uint32_t k_row, v_row;
+  // finds key l & 31's page a step before its rows are asked for
+  int pg = 0, off = 0;
   auto find_rows = [&](int key0) {
-    const int key = min(key0 + (lane & 31), k_end - 1);
-    int p, r;
-    page_of(key, a.page, inv_page, p, r);
-    const int at = min(max(table[p], 0), a.n_pages - 1);
-    k_row = (uint32_t)((at * a.kc_p + r * a.kc_t) >> 3);
-    v_row = (uint32_t)((at * a.vc_p + r * a.vc_t) >> 3);
+    int p;
+    page_of(min(key0 + (lane & 31), k_end - 1), a.page, inv_page, p, off);
+    pg = table[p];
   };
-  u32x4_t kf[2][KSTEPS], vf[NV];
-  auto load = [&](int key0) {
-    find_rows(key0);
+  uint32_t k_row, v_row;
+  u32x4_t kf[2][KSTEPS];
+  auto load_keys = [&]() {
+    const uint32_t at = min(max(pg, 0), a.n_pages - 1);
+    k_row = at * k_page + off * k_tok, v_row = at * v_page + off * v_tok;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const uint8_t* p = kbase + (uint64_t)(uint32_t)__shfl((int)k_row, 16 * m + col) * 16;
 #pragma unroll
       for (int i = 0; i < KSTEPS; ++i) kf[m][i] = *(const u32x4_t*)(p + 64 * i);
     }
+  };
+  auto copy_values = [&]() {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int r = i * KPI + lane / LPR;
-      const uint8_t* p = vbase + (uint64_t)(uint32_t)__shfl((int)v_row, r) * 16;
-      vf[i] = *(const u32x4_t*)p;
-      // (a key past the end repeats the last one, weighted 0: not its value,
-      // which may be infinite)
-      if (key0 + r >= k_end) vf[i] = u32x4_t{0, 0, 0, 0};
+      const int r = i * RPI + lane / PPR;
+      dma16(vbase + (uint64_t)((uint32_t)__shfl((int)v_row, r) + (uint64_t)((lane % PPR) ^ row_key<D>(r))) * 16, vt_lds + i * 1024);
     }
   };
 
@@ -228,30 +239,33 @@ __global__ __launch_bounds__(256) void few_kernel(const AttentionArgs a) {
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m_run = -__builtin_inff(), l_run = 0.f;
+  constexpr int STEP = kWaves * kKeys;
   int key0 = k_begin + wave * kKeys;
-  if (key0 < k_end) load(key0);
-  for (; key0 < k_end; key0 += kWaves * kKeys) {
-    const bool masked = key0 + kKeys > min(vis_all, k_end);
-    bool bad = false;
+  if (key0 < k_end) {
+    find_rows(key0);
+    load_keys();
+    copy_values();
+    find_rows(key0 + STEP);
+  }
+  // one step; MASKED: some of its keys are not seen by every row
+  auto step = [&](auto tag) {
+    constexpr bool MASKED = decltype(tag)::value;
+    const bool more = key0 + STEP < k_end;
+    f32x4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      *(u32x4_t*)(vt + (i * KPI + lane / LPR) * v_stride<D>() + 16 * (lane % LPR)) = vf[i];
-      if (masked) bad |= nonfinite8<Act>(vf[i]);
+    for (int i = 0; i < KSTEPS; ++i)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) s[m] = mfma<Act>(kf[m][i], q[i], s[m]);
+    GDNR_WAIT_VMCNT(0);  // the step's values are in LDS
+    if (more) {
+      load_keys();
+      find_rows(key0 + 2 * STEP);
     }
-    f32x4_t s[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      s[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < KSTEPS; ++i) s[m] = mfma<Act>(kf[m][i], q[i], s[m]);
-    }
-    if (key0 + kWaves * kKeys < k_end) load(key0 + kWaves * kKeys);
     float x[8], top = -__builtin_inff();
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       x[e] = s[e >> 2][e & 3] * a.scale_log2;
-      const int key = key0 + 16 * (e >> 2) + 4 * grp + (e & 3);
-      if (masked && key >= min(vis, k_end)) x[e] = -__builtin_inff();
+      if (MASKED && key0 + 16 * (e >> 2) + 4 * grp + (e & 3) >= vis) x[e] = -__builtin_inff();
       top = fmaxf(top, x[e]);
     }
     top = column_max(top);
@@ -267,36 +281,57 @@ __global__ __launch_bounds__(256) void few_kernel(const AttentionArgs a) {
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - base), l_run += p[e];
-    if (__any(bad)) {
-      // a value that some rows must not see is infinite or NaN, and a product
-      // with its weight 0 would show it to them: this step key by key
+    bool bad = false;
+    if constexpr (MASKED) {
 #pragma nounroll
-      for (int key = 0; key < kKeys; ++key) {
-        float pk = 0.f;
+      for (int i = lane; i < kKeys * PPR; i += 64) bad |= nonfinite8<Act>(*(const u32x4_t*)(vt + 16 * i));
+      bad = __any(bad);
+      if (bad) {
+        // a value that some rows must not see is infinite or NaN, and a product
+        // with its weight 0 would show it to them: this step key by key
+#pragma nounroll
+        for (int key = 0; key < kKeys; ++key) {
+          float pk = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (4 * (key >> 4) + (key & 3) == e) pk = p[e];
-        pk = __shfl(pk, col + 16 * ((key >> 2) & 3));
-        const uint32_t seen = key0 + key < min(vis, k_end) ? ~0u : 0u;
+          for (int e = 0; e < 8; ++e)
+            if (4 * (key >> 4) + (key & 3) == e) pk = p[e];
+          pk = __shfl(pk, col + 16 * ((key >> 2) & 3));
+          const uint32_t seen = key0 + key < vis ? ~0u : 0u;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          const uint2 w = *(const uint2*)(vt + key * v_stride<D>() + 32 * i + 8 * grp);
-          const float2 lo = Act::from_pair(w.x & seen), hi = Act::from_pair(w.y & seen);
-          add_in_place(o[i], pk, f32x4_t{lo.x, lo.y, hi.x, hi.y});
+          for (int i = 0; i < DT; ++i) {
+            const uint2 w = *(const uint2*)(vt + key * 2 * D + 16 * ((2 * i + (grp >> 1)) ^ row_key<D>(key)) + 8 * (grp & 1));
+            const float2 lo = Act::from_pair(w.x & seen), hi = Act::from_pair(w.y & seen);
+            add_in_place(o[i], pk, f32x4_t{lo.x, lo.y, hi.x, hi.y});
+          }
         }
       }
-      continue;
     }
-    // (the sum is of the unrounded weights; rounding them to the cache's type
-    // costs the output about its own rounding)
-    const u32x4_t pf = {pack2<Act>(p[0], p[1]), pack2<Act>(p[2], p[3]), pack2<Act>(p[4], p[5]), pack2<Act>(p[6], p[7])};
+    if (!bad) {
+      // (the sum is of the unrounded weights; rounding them to the cache's type
+      // costs the output about its own rounding)
+      const u32x4_t pf = {pack2<Act>(p[0], p[1]), pack2<Act>(p[2], p[3]), pack2<Act>(p[4], p[5]), pack2<Act>(p[6], p[7])};
+      uint32_t v_key = row_key<D>(4 * grp + (col >> 2)) ^ ((col & 3) >> 1);
+      asm volatile("" : "+v"(v_key));  // (addresses formed here, not kept)
+      const uint8_t* vl = vt + (4 * grp + (col >> 2)) * 2 * D + 8 * (col & 1);
 #pragma unroll
-    for (int i = 0; i < DT; ++i) {
-      const uint8_t* at = vt + (4 * grp + (col >> 2)) * v_stride<D>() + 32 * i + 8 * (col & 3);
-      const uint2 lo = transposed4(at), hi = transposed4(at + 16 * v_stride<D>());
-      o[i] = mfma<Act>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf, o[i]);
+      for (int i0 = 0; i0 < DT; i0 += 4) {
+        uint2 lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* at = vl + 16 * ((2 * (i0 + i)) ^ v_key);
+          lo[i] = transposed4(at), hi[i] = transposed4(at + 32 * D);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i0 + i] = mfma<Act>(u32x4_t{lo[i].x, lo[i].y, hi[i].x, hi[i].y}, pf, o[i0 + i]);
+      }
     }
-  }
+    if (more) {
+      GDNR_WAIT_LGKM0();  // the step's values have been read
+      copy_values();
+    }
+  };
+  for (; key0 + kKeys <= vis_all; key0 += STEP) step(std::false_type{});
+  for (; key0 < k_end; key0 += STEP) step(std::true_type{});
   l_run = column_sum(l_run);
 
   // join the waves: every row's sums at the largest maximum
@@ -338,12 +373,6 @@ __global__ __launch_bounds__(256) void few_kernel(const AttentionArgs a) {
     p[0] = top, p[1] = l;
   }
 }
-
-// 16-byte piece p of row r of a tile of D-element rows in LDS lies at p ^ key:
-// 16 rows' pieces then fall on distinct banks (rows of 128 bytes lie two to a
-// bank window)
-template <int D>
-__device__ __forceinline__ int row_key(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
 
 template <int D>
 struct Tile {
@@ -649,15 +678,33 @@ __global__ __launch_bounds__(256) void join_kernel(const AttentionArgs a) {
   const int vis = visible(sq, t), pieces = (vis + piece - 1) / piece;
   constexpr int E = D / 64;
   float acc[E] = {}, top = -__builtin_inff(), l = 0.f;
-  for (int z = 0; z < pieces; ++z) {
-    const int64_t at = ((int64_t)z * a.T + t) * a.HQ + h;
-    const float m = a.part_ml[2 * at], lz = a.part_ml[2 * at + 1];
-    const float m_new = fmaxf(top, m);
-    const float fo = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(top - m_new);
-    const float fz = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-    l = l * fo + lz * fz;
+  const int64_t row0 = (int64_t)t * a.HQ + h, step = (int64_t)a.T * a.HQ;
+  for (int z0 = 0; z0 < pieces; z0 += 64) {
+    // a lane a piece: its maximum and sum; then the pieces' outputs, eight in flight
+    const int z = z0 + lane, count = min(64, pieces - z0);
+    const float2 ml = z < pieces ? *(const float2*)(a.part_ml + 2 * (row0 + z * step)) : make_float2(-__builtin_inff(), 0.f);
+    float m_new = fmaxf(top, ml.x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * fo + fz * a.part[at * D + E * lane + e];
+    for (int d = 1; d < 64; d *= 2) m_new = fmaxf(m_new, __shfl_xor(m_new, d));
+    const float base = m_new == -__builtin_inff() ? 0.f : m_new;
+    const float fo = __builtin_amdgcn_exp2f(top - base), fz = z < pieces ? __builtin_amdgcn_exp2f(ml.x - base) : 0.f;
+    l = l * (z0 ? fo : 0.f) + wave_sum(fz * ml.y);
+    const float* p = a.part + (row0 + z0 * step) * D + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= z0 ? fo : 0.f;
+    for (int i0 = 0; i0 < count; i0 += 8) {
+      float x[8][E];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[i][e] = p[min(i0 + i, count - 1) * step * D + e];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = i0 + i < count ? __shfl(fz, i0 + i) : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = i0 + i < count ? fmaf(f, x[i][e], acc[e]) : acc[e];
+      }
+    }
     top = m_new;
   }
   const float norm = vis == 0 ? 0.f : 1.f / l;
@@ -674,7 +721,8 @@ template <class Act, int D>
 int launch_dim(const AttentionArgs& a, hipStream_t s) {
   const auto grid = [&](int rows, int pieces) {  // key heads first: a head's workgroups share an XCD
     const int gt = a.G < rows ? a.G : rows, tb = rows / gt;
-    return dim3(a.HKV * ((a.G + rows - 1) / rows), a.T / tb + a.N, pieces);
+    const bool one_tile = rows == kRows && a.few_rows == kRows;
+    return dim3(a.HKV * ((a.G + rows - 1) / rows), one_tile ? a.N : a.T / tb + a.N, pieces);
   };
   const auto launch = [&](auto kernel, int rows, int pieces, int lds) {
     if (lds > 64 * 1024) {  // (enabled per kernel and device; idempotent, cheap)
@@ -709,16 +757,15 @@ int launch_act(const AttentionArgs& a, hipStream_t s) {
 // piece. The lengths are on the device; the host knows their number and sum.
 // Where a sequence has 16 rows or fewer on average, few_kernel takes all of
 // them; a single longer one is tile_kernel's; otherwise each takes its kind. A
-// context is cut while a kernel would have fewer than four (few) or two (tile)
-// workgroups a compute unit, into whole steps of 128 keys, at least 256: a
-// shorter piece costs as much to join as to walk.
+// context is cut while a kernel would have fewer than eight (few) or two
+// (tile) workgroups a compute unit, into whole steps of 128 keys, at least 256:
+// a shorter piece costs as much to join as to walk.
 void plan_attention(AttentionArgs* a) {
   const int64_t cus = device_cus(), rows = (int64_t)a->T * (a->G < kRows ? a->G : kRows);
   const bool all_few = rows <= (int64_t)kRows * a->N, all_tile = !all_few && a->N == 1;
   a->few_rows = all_few ? INT32_MAX : all_tile ? 0 : kRows;
-  const auto plan = [&](int kind, int tile_rows, int64_t want) {
-    const int64_t gt = a->G < tile_rows ? a->G : tile_rows, tb = tile_rows / gt;
-    const int64_t groups = (a->T / tb + a->N) * a->HKV * ((a->G + tile_rows - 1) / tile_rows);
+  const auto plan = [&](int kind, int64_t tiles, int64_t want) {
+    const int64_t groups = tiles * a->HKV;
     int64_t p = a->max_context;
     if (groups < want) p = (a->max_context * groups + want - 1) / want;
     p = (p + 127) / 128 * 128;
@@ -726,9 +773,13 @@ void plan_attention(AttentionArgs* a) {
     a->piece[kind] = (int32_t)(p < INT32_MAX ? p : INT32_MAX);
     a->pieces[kind] = a->max_context ? (int32_t)((a->max_context + p - 1) / p) : 1;
   };
+  const auto tiles_of = [&](int tile_rows) {
+    const int64_t gt = a->G < tile_rows ? a->G : tile_rows;
+    return (a->T / (tile_rows / gt) + 1) * ((a->G + tile_rows - 1) / tile_rows);
+  };
   a->pieces[0] = a->pieces[1] = 0;
-  if (!all_tile) plan(0, kRows, 4 * cus);
-  if (!all_few) plan(1, a->D == 256 ? 64 : 128, 2 * cus);
+  if (!all_tile) plan(0, all_few && a->T > a->N ? tiles_of(kRows) : (int64_t)a->N * ((a->G + kRows - 1) / kRows), 8 * cus);
+  if (!all_few) plan(1, tiles_of(a->D == 256 ? 64 : 128), 2 * cus);
 }
 
 int launch_attention(const AttentionArgs& a, int act_dt, void* stream) {
