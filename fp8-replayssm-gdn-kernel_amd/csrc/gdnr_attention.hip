@@ -453,12 +453,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   auto copy = [&](int buf) {
     const uint32_t at = min(max(pg, 0), a.n_pages - 1);
     const uint32_t k_row = at * k_page + off * k_tok, v_row = at * v_page + off * v_tok;
+    uint32_t kr[COPIES], vr[COPIES];
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
-      const int from = i * RPI + lane / PPR, piece16 = (lane % PPR) ^ row_key<D>((i * kWaves + wave) * RPI + lane / PPR);
+      const int from = i * RPI + lane / PPR;
+      kr[i] = (uint32_t)__shfl((int)k_row, from), vr[i] = (uint32_t)__shfl((int)v_row, from);
+    }
+    GDNR_COMPILER_FENCE();
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const uint64_t piece16 = (lane % PPR) ^ row_key<D>((i * kWaves + wave) * RPI + lane / PPR);
       const uint32_t to = lds0 + buf * 2 * TL::KB + i * kWaves * 1024;
-      dma16(kbase + (uint64_t)((uint32_t)__shfl((int)k_row, from) + (uint64_t)piece16) * 16, to);
-      dma16(vbase + (uint64_t)((uint32_t)__shfl((int)v_row, from) + (uint64_t)piece16) * 16, to + TL::KB);
+      dma16(kbase + (kr[i] + piece16) * 16, to);
+      dma16(vbase + (vr[i] + piece16) * 16, to + TL::KB);
     }
   };
 
@@ -481,10 +488,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     constexpr bool MASKED = decltype(tag)::value;
     GDNR_WAIT_VMCNT(0);
     __syncthreads();  // the step's keys and values are in LDS; the other buffer is no longer read
-    if (key0 + KEYS < k_end) {
-      copy(buf ^ 1);
-      if (key0 + 2 * KEYS < k_end) find_rows(key0 + 2 * KEYS);
-    }
     const uint8_t* kt = lds + buf * 2 * TL::KB;
     const uint8_t* vt = kt + TL::KB;
     // (the fragments' addresses are formed where they are used: kept across
@@ -508,6 +511,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
     };
     read_keys(0);
+    GDNR_COMPILER_FENCE();
+    if (key0 + KEYS < k_end) {
+      copy(buf ^ 1);
+      if (key0 + 2 * KEYS < k_end) find_rows(key0 + 2 * KEYS);
+    }
+    GDNR_COMPILER_FENCE();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int st = 0; st < STAGES; ++st) {
       if (st + 1 < STAGES) read_keys(st + 1);
@@ -523,6 +533,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                                           i + h == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : s[2 * m2 + m][nt]);
     }
     GDNR_COMPILER_FENCE();
+    __builtin_amdgcn_s_setprio(0);
     // the values' fragments of 32 keys, read before the weights are formed
     u32x4_t vf[DT];
     auto read_values = [&](int half) {
@@ -619,6 +630,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     // O^T += V^T P^T. (The sum is of the unrounded weights; rounding them to
     // the cache's type costs the output about its own rounding.)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int half = 0; half < MT / 2; ++half) {
       u32x4_t pf[NT];
@@ -637,6 +649,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         GDNR_COMPILER_FENCE();
       }
     }
+    __builtin_amdgcn_s_setprio(0);
   };
   for (; key0 + KEYS <= vis_all; key0 += KEYS, buf ^= 1) step(std::false_type{});
   for (; key0 < k_end; key0 += KEYS, buf ^= 1) step(std::true_type{});
