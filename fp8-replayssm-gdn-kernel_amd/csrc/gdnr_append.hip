@@ -48,7 +48,21 @@ __device__ __forceinline__ u32x4_t pack8(const float* f) {
   return u32x4_t{w[0], w[1], w[2], w[3]};
 }
 
-template <class Act, int D>
+// 4 N floats from p (4-byte aligned; 16 bytes an instruction)
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float* f) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const f32x4_a4 x = ((const f32x4_a4*)p)[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[4 * i + j] = x[j];
+  }
+}
+
+constexpr int kAhead = 4;  // groups of heads a wave asks for at once
+
+template <class Act, int D, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
   constexpr int LPH = D / 8;       // lanes per head
   constexpr int HPW = 64 / LPH;    // heads a wave instruction moves
@@ -57,83 +71,128 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
   const int t = (int)(unit / a.splits), part = (int)(unit - (int64_t)t * a.splits);
   if (t >= a.T) return;  // wave-uniform
   const int cl = lane & (LPH - 1), sub = lane / LPH;
-  const int heads = a.HQ + 2 * a.HKV;
   const int pos = min(max(__builtin_amdgcn_readfirstlane(a.position[t * a.po_s]), 0), a.positions - 1);
   const int slot = __builtin_amdgcn_readfirstlane(a.slot[t * a.sl_s]);
   const bool kept = slot >= 0 && slot < a.slots;  // any other slot appends nothing
   const int page = kept ? slot / a.page : 0, at = kept ? slot - page * a.page : 0;
 
-  // cosines and signed sines of this lane's elements; a lane past the rotary
-  // part turns by nothing
+  // this lane's elements, and its partner's that they turn with
   const int half = a.rotary / 2, e0 = 8 * cl;
-  const bool turned = e0 < a.rotary;
-  float c[8], s[8];
-  if (turned) {
-    const float* row = a.table + pos * a.tb_p;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = a.interleaved ? (e0 + e) >> 1 : (e0 < half ? e0 + e : e0 + e - half);
-      c[e] = row[i];
-      const float sine = row[half + i];
-      s[e] = (a.interleaved ? !(e & 1) : e0 < half) ? -sine : sine;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = 1.f, s[e] = 0.f;
-  }
-  const int partner = a.interleaved || !turned ? lane : (e0 < half ? lane + half / 8 : lane - half / 8);
+  const bool turned = e0 < a.rotary, low = e0 < half;
+  const int partner = INTERLEAVED || !turned ? lane : (low ? lane + half / 8 : lane - half / 8);
   const int ep = 8 * (partner & (LPH - 1));
+  // its cosines and signed sines
+  float c[8], s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = 1.f, s[e] = 0.f;
+  if (turned) {
+    const float* angles = a.table + pos * a.tb_p;
+    if constexpr (INTERLEAVED) {
+      float x[4], y[4];
+      load_floats<1>(angles + e0 / 2, x);
+      load_floats<1>(angles + half + e0 / 2, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] = x[e >> 1], s[e] = (e & 1) ? y[e >> 1] : -y[e >> 1];
+    } else {
+      const float* own = angles + (low ? e0 : e0 - half);
+      load_floats<2>(own, c);
+      load_floats<2>(own + half, s);
+      if (low) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = -s[e];
+      }
+    }
+  }
 
-  for (int head = part * HPW; head < heads; head += a.splits * HPW) {
-    const int hh = head + sub;
-    const bool on = hh < heads, is_q = hh < a.HQ, is_k = !is_q && hh < a.HQ + a.HKV;
-    const uint8_t* src = !on ? nullptr
-                         : is_q ? (const uint8_t*)a.q + (t * a.q_t + hh * a.q_h) * 2
-                         : is_k ? (const uint8_t*)a.k + (t * a.k_t + (hh - a.HQ) * a.k_h) * 2
-                                : (const uint8_t*)a.v + (t * a.v_t + (hh - a.HQ - a.HKV) * a.v_h) * 2;
-    u32x4_t w = {0, 0, 0, 0};
-    if (on) w = *(const u32x4_t*)(src + 16 * cl);
-    if (head < a.HQ + a.HKV) {  // wave-uniform: some head of these is q or k
-      u32x4_t wp;
+  const int q_groups = (a.HQ + HPW - 1) / HPW, kv_groups = (a.HKV + HPW - 1) / HPW;
+  // one kind of heads: its rows in groups of HPW heads, group `first` and every
+  // `splits`-th from there
+  auto heads_of = [&](const void* from, int64_t from_t, int64_t from_h, void* to, int64_t to_row, int64_t to_h, int heads,
+                      int first, const float* weight, bool rotate) {
+    const int groups = (heads + HPW - 1) / HPW;
+    if (first >= groups) return;
+    const uint8_t* src = (const uint8_t*)from + (t * from_t + sub * from_h + e0) * 2;
+    uint8_t* dst = (uint8_t*)to + (to_row + sub * to_h + e0) * 2;
+    u32x4_t w[kAhead];
+    auto ask = [&](int g0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) wp[i] = (uint32_t)__shfl((int)w[i], partner);
-      float x[8], xp[8], y[8], sq = 0.f;
-      unpack8<Act>(w, x);
-      unpack8<Act>(wp, xp);
-      const float* weight = is_q ? a.q_weight : a.k_weight;
-      const bool norm = weight != nullptr && (is_q || is_k);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sq = fmaf(x[e], x[e], sq);
-      const float r = 1.f / sqrtf(group_sum<LPH>(sq) * (1.f / D) + a.eps);
-      if (norm) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= r * weight[e0 + e], xp[e] *= r * weight[ep + e];
+      for (int u = 0; u < kAhead; ++u) {
+        const int g = g0 + u * a.splits;
+        w[u] = u32x4_t{0, 0, 0, 0};
+        if (g * HPW + sub < heads) w[u] = *(const u32x4_t*)(src + g * HPW * from_h * 2);
+      }
+    };
+    ask(first);
+    // y = r (x cw + x_partner sw): the weight, cosine and signed sine in one
+    float cw[8], sw[8];
+    if (rotate) {
+      float own[8], other[8];
+      if (weight) {
+        load_floats<2>(weight + e0, own);
+        load_floats<2>(weight + ep, other);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float other = a.interleaved ? x[e ^ 1] : xp[e];
-        y[e] = turned ? fmaf(other, s[e], x[e] * c[e]) : x[e];
+        const int o = INTERLEAVED ? e ^ 1 : e;
+        cw[e] = weight ? own[e] * c[e] : c[e], sw[e] = weight ? other[o] * s[e] : s[e];
       }
-      if (is_q || is_k) w = pack8<Act>(y);
     }
-    if (is_q) {
-      *(u32x4_t*)((uint8_t*)a.q_out + (t * a.qo_t + hh * a.qo_h) * 2 + 16 * cl) = w;
-    } else if (on && kept) {
-      uint8_t* dst = is_k ? (uint8_t*)a.k_cache + (page * a.kc_p + at * a.kc_t + (hh - a.HQ) * a.kc_h) * 2
-                          : (uint8_t*)a.v_cache + (page * a.vc_p + at * a.vc_t + (hh - a.HQ - a.HKV) * a.vc_h) * 2;
-      *(u32x4_t*)(dst + 16 * cl) = w;
+    for (int g0 = first; g0 < groups; g0 += kAhead * a.splits) {
+      if (g0 != first) ask(g0);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int g = g0 + u * a.splits;
+        if (g >= groups) break;  // wave-uniform
+        if (rotate) {
+          float x[8], z[8], sq = 0.f, r = 1.f;
+          unpack8<Act>(w[u], x);
+          if constexpr (INTERLEAVED) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = x[e ^ 1];
+          } else {
+            u32x4_t wp;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wp[i] = (uint32_t)__shfl((int)w[u][i], partner);
+            unpack8<Act>(wp, z);
+          }
+          if (weight) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sq = fmaf(x[e], x[e], sq);
+            r = 1.f / sqrtf(group_sum<LPH>(sq) * (1.f / D) + a.eps);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= cw[e];
+          if (turned) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = fmaf(z[e], sw[e], x[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= r;
+          w[u] = pack8<Act>(x);
+        }
+        if (g * HPW + sub < heads) *(u32x4_t*)(dst + g * HPW * to_h * 2) = w[u];
+      }
     }
-  }
+  };
+  heads_of(a.q, a.q_t, a.q_h, a.q_out, t * a.qo_t, a.qo_h, a.HQ, part, a.q_weight, true);
+  if (!kept) return;
+  // (the groups go round: the kinds' first ones fall to different waves)
+  const int k_first = (part + a.splits - q_groups % a.splits) % a.splits;
+  const int v_first = (k_first + a.splits - kv_groups % a.splits) % a.splits;
+  heads_of(a.k, a.k_t, a.k_h, a.k_cache, page * a.kc_p + at * a.kc_t, a.kc_h, a.HKV, k_first, a.k_weight, true);
+  heads_of(a.v, a.v_t, a.v_h, a.v_cache, page * a.vc_p + at * a.vc_t, a.vc_h, a.HKV, v_first, nullptr, false);
 }
 
 template <class Act, int D>
 int launch_append_dim(AppendArgs a, hipStream_t s) {
   // waves for every compute unit twice over, while a wave still has heads
-  const int heads = a.HQ + 2 * a.HKV, most = (heads + 512 / D - 1) / (512 / D);
+  constexpr int HPW = 512 / D;
+  const int most = (a.HQ + HPW - 1) / HPW + 2 * ((a.HKV + HPW - 1) / HPW);
   const int want = (int)((8 * (int64_t)device_cus() + a.T - 1) / a.T);
   a.splits = want < 1 ? 1 : want < most ? want : most;
-  const int64_t units = (int64_t)a.T * a.splits;
-  hipLaunchKernelGGL((append_kernel<Act, D>), dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, s, a);
+  const dim3 grid((uint32_t)(((int64_t)a.T * a.splits + 3) / 4));
+  if (a.interleaved) hipLaunchKernelGGL((append_kernel<Act, D, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((append_kernel<Act, D, false>), grid, dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
 
