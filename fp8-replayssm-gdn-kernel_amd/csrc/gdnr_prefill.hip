@@ -239,15 +239,16 @@ __device__ __forceinline__ f32x4_t product(const Operand<SPLIT>& a, const Operan
 }
 
 // Workspace: per chunk slot and key head the unit keys and queries [C][K] f16
-// (SPLIT: high, then low), a row's pieces as unit_at places them; per slot and value head the operand tiles of T - I
-// and A (64 lanes x 16 bytes each; SPLIT: high, then low) and the tokens'
-// {beta}[C], {e^G}[C], {e^(G_C - G)}[C], {-beta e^G}[C], first bad token (an
-// int), padded to 2 KiB.
-// Sequence n's chunks take the slots from cu[n] / C + n on.
-constexpr int kScalars = 4 * C + 4;
-__host__ __device__ constexpr int64_t unit_bytes(bool split) { return 2 * C * K * 2 * (split ? 2 : 1); }
-__host__ __device__ constexpr int64_t tile_bytes(bool split) { return 2 * kTri * 1024 * (split ? 2 : 1); }
-__host__ __device__ constexpr int64_t head_bytes(bool split) { return tile_bytes(split) + 2048; }
+// (SPLIT: high, then low), a row's pieces as unit_at places them; per slot and
+// value head the tokens' {beta}[C], {-beta e^G}[C], {e^(G_C - G)}[C], {e^G}[C],
+// first bad token (an int), padded to 2 KiB, then the operand tiles of T - I and
+// of A (64 lanes x 16 bytes each; SPLIT: high, then low). Sequence n's chunks take
+// the slots from cu[n] / C + n on.
+constexpr int kScalars = 2048;
+__host__ __device__ constexpr int64_t plane_bytes(bool split) { return C * K * 2 * (split ? 2 : 1); }  // keys, or queries
+__host__ __device__ constexpr int64_t unit_bytes(bool split) { return 2 * plane_bytes(split); }
+__host__ __device__ constexpr int64_t tri_bytes(bool split) { return kTri * 1024 * (split ? 2 : 1); }
+__host__ __device__ constexpr int64_t head_bytes(bool split) { return kScalars + 2 * tri_bytes(split); }
 
 struct Work {
   uint8_t* unit;  // [slots][H]
@@ -265,9 +266,6 @@ __host__ __device__ inline Work work_of(const PrefillArgs& a, bool split) {
 __host__ __device__ constexpr int unit_at(int t, int k4) {
   return 2 * K * t + 16 * ((4 * (k4 >> 3) + (k4 & 3)) ^ (t & 15)) + 8 * ((k4 >> 2) & 1);
 }
-
-// chunks whose operands the scan keeps in LDS
-__host__ __device__ constexpr int scan_buffers(bool split) { return split ? 1 : 2; }
 
 // index of the tile (16 rows of t, 32 columns of i) in a lower triangle
 __host__ __device__ constexpr int tri(int tt, int ts) { return tt < 2 ? tt : 2 * (tt - 1) + ts; }
@@ -407,16 +405,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
       const double last = __shfl(G, 63);
       Gs[wave][t] = G;
       betas[wave][t] = beta;
-      float* sc = (float*)(w.head + ((int64_t)slot * a.HV + hv) * head_bytes(SPLIT) + tile_bytes(SPLIT));
+      float* sc = (float*)(w.head + ((int64_t)slot * a.HV + hv) * head_bytes(SPLIT));
+      const float grow = exp2_diff<SPLIT>(G);
       sc[t] = beta;
-      sc[C + t] = exp2_diff<SPLIT>(G);
+      sc[C + t] = -beta * grow * (SPLIT ? 1.f / kFix : 1.f);
       sc[2 * C + t] = exp2_diff<SPLIT>(last - G);
-      sc[3 * C + t] = -beta * exp2_diff<SPLIT>(G) * (SPLIT ? 1.f / kFix : 1.f);
+      sc[3 * C + t] = grow;
       if (t == 0) ((int*)sc)[4 * C] = first;
     }
     __syncthreads();
     for (int e = 0; e < heads; ++e) {
-      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + e) * head_bytes(SPLIT);
+      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + e) * head_bytes(SPLIT) + kScalars;
       const int t = 16 * wave + col;
       const double Gt = Gs[e][t];
       const float bt = betas[e][t];
@@ -490,7 +489,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(-tl[j], y[j], x[c], 0, 0, 0);
       }
-      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + e) * head_bytes(SPLIT);
+      uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + e) * head_bytes(SPLIT) + kScalars;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -524,22 +523,51 @@ __device__ __forceinline__ float column_max(float x) {
   return __builtin_elementwise_maximum(__uint_as_float(row[0]), __uint_as_float(row[1]));
 }
 
-// A sequence's chunks in order, for 16 NV V-rows of one value head a wave,
-// WAVES waves sharing a chunk's operands in LDS. A wave's V-rows are the
-// columns (lane & 15) of every product, so what one product leaves in
-// registers (rows k or t: 4 grp + j of a 16-row tile) is the next one's
-// operand as it stands: both operands of a product may take its contraction in
-// any order, and the keys', T's and A's fragments are read in that one.
-template <class Act, class St, bool SPLIT, int WAVES, int NV>
+// KIB KiB (an even number) from memory to LDS, by COUNT waves of which this is wave w
+template <int KIB, int COUNT>
+__device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, int w) {
+#pragma unroll
+  for (int i = 0; i < (KIB + 4 * COUNT - 1) / (4 * COUNT); ++i) {
+    const int x = i * COUNT + w;  // wave-uniform
+    if (x < KIB / 4) dma_kib<4>(src + x * 4096, lds_addr + x * 4096);
+    else if (KIB % 4 && x == KIB / 4) dma_kib<2>(src + x * 4096, lds_addr + x * 4096);
+  }
+}
+
+// LDS of the scan: a chunk's keys, scalars and T tiles twice (the next chunk's
+// arrive while this one's are used), its queries and A tiles twice, or once
+// under SPLIT, whose operands are twice as large; with ROLES the scalars again
+// beside the queries, and twice what the state's wave hands over.
+template <bool SPLIT, bool ROLES>
+struct ScanLds {
+  static constexpr int KEYS = (int)(plane_bytes(SPLIT) + kScalars + tri_bytes(SPLIT));
+  static constexpr int QUERIES = (int)(plane_bytes(SPLIT) + tri_bytes(SPLIT)) + (ROLES ? kScalars : 0);
+  static constexpr int QBUFS = SPLIT ? 1 : 2;
+  static constexpr int HANDED = ROLES ? 7 * 1024 : 0;  // 4 operands of S, 2 of U, scale and first bad token
+  static constexpr int BYTES = 2 * KEYS + QBUFS * QUERIES + 2 * HANDED;
+};
+
+// A sequence's chunks in order. A wave has 16 V-rows of one value head, the
+// columns (lane & 15) of every product, so what one product leaves in registers
+// (rows k or t: 4 grp + j of a 16-row tile) is the next one's operand as it
+// stands: both operands of a product may take its contraction in any order, and
+// the keys', queries', T's and A's fragments are read in that one.
+//
+// The chain over the chunks is the state's: K S0^T, R, U, S1. The outputs hang
+// off it. With ROLES (two waves a workgroup) one wave carries the chain and
+// hands S0's and U's operands through LDS to a second one, which forms the
+// outputs of chunk c while the first is at chunk c + 1; otherwise WAVES waves
+// do both for 16 V-rows each on shared operands.
+template <class Act, class St, bool SPLIT, int WAVES, bool ROLES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_scan_kernel(const PrefillArgs a) {
-  constexpr int ES = Act::kBytes, P = SPLIT ? 2 : 1, RS = 2 * K;
-  constexpr int kUnits = 2 * P * C * RS;
-  constexpr int kHead = (int)head_bytes(SPLIT), kBuf = kUnits + kHead;
-  constexpr int BUFS = scan_buffers(SPLIT);
+  using L = ScanLds<SPLIT, ROLES>;
+  constexpr int ES = Act::kBytes, P = SPLIT ? 2 : 1, RS = 2 * K, COLS = ROLES ? 16 : 16 * WAVES;
+  constexpr float kUp = SPLIT ? kFix : 1.f, kDown = 1.f / kUp;
+  static_assert(!ROLES || (WAVES == 2 && !SPLIT), "one wave a role");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  constexpr int COLS = 16 * NV * WAVES;
+  const bool chain = !ROLES || wave == 0, outputs = !ROLES || wave == 1;
   // Workgroups go to the 8 XCDs in turn: those of one key head, which read the
   // same keys and queries, to one of them.
   const int blocks = a.V / COLS, n = blockIdx.y;
@@ -548,94 +576,114 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const int per = a.G * blocks, j = unit_id >> 3;
     unit_id = ((unit_id & 7) + 8 * (j / per)) * per + j % per;
   }
-  const int hv = unit_id / blocks;
-  const int v0 = (unit_id - hv * blocks) * COLS + wave * 16 * NV + col * NV;  // this lane's V-rows: v0 .. v0 + NV - 1
-  const int h = hv / a.G;
+  const int hv = unit_id / blocks, h = hv / a.G;
+  const int v0 = (unit_id - hv * blocks) * COLS + (ROLES ? 0 : wave * 16) + col;  // this lane's V-row
   int begin, end;
   sequence_rows(a, n, begin, end);
   const bool started = sequence_started(a, n);
   if (begin == end && started) return;
   const int len = end - begin, chunks = (len + C - 1) / C;
-  const uint8_t *unit, *head;  // of the next chunk to fetch
+  const uint8_t *unit, *head;  // of chunk 0
+  const int64_t unit_step = a.H * unit_bytes(SPLIT), head_step = a.HV * head_bytes(SPLIT);
   {
     const Work w = work_of(a, SPLIT);
     const int64_t slot0 = begin / C + n;
-    unit = w.unit + (slot0 * a.H + h) * unit_bytes(SPLIT);
-    head = w.head + (slot0 * a.HV + hv) * head_bytes(SPLIT);
+    unit = w.unit + slot0 * unit_step + h * unit_bytes(SPLIT);
+    head = w.head + slot0 * head_step + hv * head_bytes(SPLIT);
   }
 
-  // the state, transposed: tile kt of 16 columns k, rows 4 grp + j
-  uint8_t* sp = (uint8_t*)a.state + ((int64_t)sequence_slot(a, n) * a.st_s + hv * a.st_h + (int64_t)v0 * a.st_v + 4 * grp) * St::kBytes;
-  f32x4_t S[NV][8];  // times sc[nv]
-  float sc[NV], inv[NV];
-#pragma unroll
-  for (int nv = 0; nv < NV; ++nv) {
-    sc[nv] = inv[nv] = 1.f;
-#pragma unroll
-    for (int kt = 0; kt < 8; ++kt) {
-      Raw<St, 4> x;
-      if (started) x.load(sp + (nv * a.st_v + 16 * kt) * St::kBytes);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) S[nv][kt][j] = started ? x[j] : 0.f;
-    }
-  }
-
-  // a chunk's operands, straight from memory to LDS as they lie, 4 KiB a wave
-  // and turn (the last one 2)
-  constexpr int kRowQuads = kUnits / 4096, kQuads = kRowQuads + (kHead + 2048) / 4096;
-  static_assert(kUnits % 4096 == 0 && kHead % 4096 == 2048, "whole turns");
+  // Operands from memory to LDS as they lie.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds;
-  auto fetch = [&](int c) {
-    const uint32_t to = lds0 + (uint32_t)((c % BUFS) * kBuf);
-#pragma unroll
-    for (int i = 0; i < (kQuads + WAVES - 1) / WAVES; ++i) {
-      const int x = i * WAVES + wave;  // wave-uniform
-      if (x < kRowQuads) dma_kib<4>(unit + x * 4096, to + x * 4096);
-      else if (x < kQuads - 1) dma_kib<4>(head + (x - kRowQuads) * 4096, to + x * 4096);
-      else if (x == kQuads - 1) dma_kib<2>(head + (x - kRowQuads) * 4096, to + x * 4096);
-    }
-    unit += a.H * unit_bytes(SPLIT), head += a.HV * head_bytes(SPLIT);
+  constexpr int kTeam = ROLES ? 1 : WAVES;  // waves that fetch a part
+  const int member = ROLES ? 0 : wave;
+  auto fetch_keys = [&](int c) {
+    const uint32_t to = lds0 + (c & 1) * L::KEYS;
+    dma_part<(int)plane_bytes(SPLIT) / 1024, kTeam>(unit + c * unit_step, to, member);
+    dma_part<(int)(kScalars + tri_bytes(SPLIT)) / 1024, kTeam>(head + c * head_step, to + plane_bytes(SPLIT), member);
   };
-  // the chunk's v: rows t of this lane, NV neighbours each, as raw bits
-  using VBits = typename std::conditional<NV == 2, typename Act::Pair, typename Act::Bits>::type;
-  VBits vn[16];
+  auto queries_at = [&](int c) { return 2 * L::KEYS + (L::QBUFS == 2 ? (c & 1) * L::QUERIES : 0); };
+  auto fetch_queries = [&](int c) {
+    const uint32_t to = lds0 + queries_at(c);
+    dma_part<(int)plane_bytes(SPLIT) / 1024, kTeam>(unit + c * unit_step + plane_bytes(SPLIT), to, member);
+    dma_part<(int)tri_bytes(SPLIT) / 1024, kTeam>(head + c * head_step + kScalars + tri_bytes(SPLIT), to + plane_bytes(SPLIT), member);
+    if constexpr (ROLES) dma_part<kScalars / 1024, kTeam>(head + c * head_step, to + plane_bytes(SPLIT) + tri_bytes(SPLIT), member);
+  };
+  // 16 tokens by 32 columns k of keys or queries at b
+  auto rows_of = [&](const uint8_t* b, int tile, int step) {
+    Operand<SPLIT> o;
+    const uint8_t* p = b + (16 * tile + col) * RS + 16 * ((4 * step + grp) ^ col);
+    o.hi = *(const u32x4_t*)p;
+    if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + C * RS);
+    return o;
+  };
+  auto triangle = [&](const uint8_t* tiles, int tt, int ts) {
+    Operand<SPLIT> o;
+    const uint8_t* p = tiles + tri(tt, ts) * 1024 + 16 * lane;
+    o.hi = *(const u32x4_t*)p;
+    if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + kTri * 1024);
+    return o;
+  };
+  // The LDS operands of a product are read a stage or more before they are
+  // used, which the fences keep the compiler from undoing: a read just before
+  // its product costs its latency some 60 times a chunk.
+  constexpr int AHEAD = SPLIT ? 1 : 2;  // k-steps of 4 fragments read before the first product
+  Operand<SPLIT> f[AHEAD + 1][4], tf[kTri], bs[4], ub[2];
+  auto read_rows = [&](const uint8_t* b, int s) {
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) f[s % (AHEAD + 1)][tt] = rows_of(b, tt, s);
+  };
+  auto read_triangle = [&](const uint8_t* tiles) {
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int s = 0; s <= tt / 2; ++s) tf[tri(tt, s)] = triangle(tiles, tt, s);
+  };
+  auto by_state = [&](const uint8_t* b, f32x4_t(&x)[4]) {  // rows 0 .. AHEAD - 1 already asked for
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (s + AHEAD < 4) read_rows(b, s + AHEAD);
+      GDNR_COMPILER_FENCE();
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) x[tt] = product<SPLIT>(f[s % (AHEAD + 1)][tt], bs[s], s == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[tt]);
+    }
+  };
+  auto by_triangle = [&](f32x4_t(&x)[4]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int tt = 2 * s; tt < 4; ++tt) x[tt] = product<SPLIT>(tf[tri(tt, s)], ub[s], x[tt]);
+  };
+
+  // the state, transposed: tile kt of 16 columns k, rows 4 grp + j; times sc
+  uint8_t* sp = (uint8_t*)a.state + ((int64_t)sequence_slot(a, n) * a.st_s + hv * a.st_h + (int64_t)v0 * a.st_v + 4 * grp) * St::kBytes;
+  f32x4_t S[8];
+  float sc = 1.f, inv = 1.f;
+  typename Act::Bits vn[16];  // the next chunk's v: rows t of this lane, as raw bits
   const int64_t v_row = a.mx_t * ES, o_row = a.o_t * ES;
   const uint8_t* vp = (const uint8_t*)a.mixed + (int64_t)begin * v_row + (2 * a.H * K + hv * a.V) * ES;
   uint8_t* op = (uint8_t*)a.out + (int64_t)begin * o_row + hv * a.o_h * ES;
   const uint32_t v_lane = (uint32_t)(4 * grp * v_row) + v0 * ES, o_lane = (uint32_t)(4 * grp * o_row) + v0 * ES;
-  auto load_v = [&](int i, const uint8_t* p) {
-    if constexpr (NV == 2) vn[i] = Act::ld_pair_bits(p);
-    else vn[i] = Act::ld_bits(p, 0);
-  };
   auto fetch_v = [&](int c) {
     const uint8_t* p = vp + c * C * v_row;
     if ((c + 1) * C <= len) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) load_v(i, p + (16 * (i >> 2) + (i & 3)) * v_row + v_lane);
+      for (int i = 0; i < 16; ++i) vn[i] = Act::ld_bits(p + (16 * (i >> 2) + (i & 3)) * v_row + v_lane, 0);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) load_v(i, p + (uint32_t)min(16 * (i >> 2) + (i & 3) + 4 * grp, len - 1 - c * C) * v_row + v0 * ES);
+      for (int i = 0; i < 16; ++i) vn[i] = Act::ld_bits(p + (uint32_t)min(16 * (i >> 2) + (i & 3) + 4 * grp, len - 1 - c * C) * v_row + v0 * ES, 0);
     }
   };
+  bool any_bad = false;
+  int first = C;  // first token of the chunk whose results are NaN in this V-row
 
-  if (chunks) {
-    fetch(0), fetch_v(0);
-    GDNR_WAIT_VMCNT(0);
-  }
-  for (int c = 0; c < chunks; ++c) {
-    // chunk c's operands are in LDS (every wave waited for its part), those of
-    // c - 1 are no longer read
-    __syncthreads();
-    const uint8_t* b = lds + (c % BUFS) * kBuf;
-    const uint8_t* tiles = b + kUnits;
-    const float* scal = (const float*)(tiles + tile_bytes(SPLIT));
-    auto rows_of = [&](int plane, int tile, int step) {  // 16 tokens by 32 columns k
-      Operand<SPLIT> o;
-      const uint8_t* p = b + (plane * C + 16 * tile + col) * RS + 16 * ((4 * step + grp) ^ col);
-      o.hi = *(const u32x4_t*)p;
-      if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + C * RS);
-      return o;
-    };
+  // the chain: chunk c's R and U from S, then S after it
+  auto state_step = [&](int c) {
+    const uint8_t* b = lds + (c & 1) * L::KEYS;
+    const float* scal = (const float*)(b + plane_bytes(SPLIT));
+    const uint8_t* tiles = b + plane_bytes(SPLIT) + kScalars;
+    const f32x4_t* beta4 = (const f32x4_t*)scal;
+    const f32x4_t* held4 = (const f32x4_t*)(scal + C);
+    const f32x4_t* end4 = (const f32x4_t*)(scal + 2 * C);
     auto turned = [&](int tile, int step) {  // 16 columns k of the keys by 32 tokens
       Operand<SPLIT> o;
       const int row = 4 * grp + (col >> 2);
@@ -649,288 +697,239 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       }
       return o;
     };
-    auto triangle = [&](int base, int tt, int ts) {
-      Operand<SPLIT> o;
-      const uint8_t* p = tiles + (base * P + tri(tt, ts)) * 1024 + 16 * lane;
-      o.hi = *(const u32x4_t*)p;
-      if constexpr (SPLIT) o.lo = *(const u32x4_t*)(p + kTri * 1024);
-      return o;
-    };
-    constexpr float kUp = SPLIT ? kFix : 1.f, kDown = 1.f / kUp;
-    const f32x4_t* beta4 = (const f32x4_t*)scal;
-    const f32x4_t* grow4 = (const f32x4_t*)(scal + C);
-    const f32x4_t* end4 = (const f32x4_t*)(scal + 2 * C);
-    const f32x4_t* held4 = (const f32x4_t*)(scal + 3 * C);
-    const float total = scal[2 * C - 1];
+    const float total = scal[4 * C - 1];
     const int bad_token = __builtin_amdgcn_readfirstlane(((const int*)scal)[4 * C]);
-
-    float v[NV][4][4];
+    float v[4][4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if constexpr (NV == 2) {
-        const float2 x = Act::from_pair(vn[i]);
-        v[0][i >> 2][i & 3] = x.x, v[1][i >> 2][i & 3] = x.y;
-      } else {
-        v[0][i >> 2][i & 3] = Act::from_bits(vn[i]);
-      }
-    }
+    for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = Act::from_bits(vn[i]);
     if ((c + 1) * C > len) {
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (c * C + 16 * (i >> 2) + 4 * grp + (i & 3) >= len) v[nv][i >> 2][i & 3] = 0.f;
+      for (int i = 0; i < 16; ++i)
+        if (c * C + 16 * (i >> 2) + 4 * grp + (i & 3) >= len) v[i >> 2][i & 3] = 0.f;
     }
     if (c + 1 < chunks) {
-      if constexpr (BUFS == 2) fetch(c + 1);
       fetch_v(c + 1);
+      GDNR_COMPILER_FENCE();
+      if constexpr (SPLIT) fetch_queries(c);
+      fetch_keys(c + 1);
+    } else if constexpr (SPLIT) {
+      fetch_queries(c);
     }
-
-    constexpr int AHEAD = SPLIT ? 1 : 2;  // k-steps of 4 fragments read before the first product
-    Operand<SPLIT> f[AHEAD + 1][4];
-    auto read_rows = [&](int plane, int s) {
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) f[s % (AHEAD + 1)][tt] = rows_of(plane, tt, s);
-    };
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) read_rows(0, s);
+    for (int s = 0; s < AHEAD; ++s) read_rows(b, s);
     GDNR_COMPILER_FENCE();
 
     // V-rows with a value that is not finite: zeros here, NaN from its token on
-    float bound[NV];  // |R| and |U| are at most 64 (|v| + 12 |S|)
-    auto largest = [&](int nv) {
+    float bound;  // |R| and |U| are at most 64 (|v| + 12 |S|)
+    auto largest = [&]() {
       float x = 0.f, x2 = 0.f, y = 0.f;
 #pragma unroll
-      for (int kt = 0; kt < 8; ++kt) x = max3_abs(x, S[nv][kt][0], S[nv][kt][1]), x2 = max3_abs(x2, S[nv][kt][2], S[nv][kt][3]);
+      for (int kt = 0; kt < 8; ++kt) x = max3_abs(x, S[kt][0], S[kt][1]), x2 = max3_abs(x2, S[kt][2], S[kt][3]);
       x = __builtin_elementwise_maximum(x, x2);
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) y = max3_abs(y, v[nv][i >> 2][i & 3], v[nv][i >> 2][(i & 3) + 1]);
-      bound[nv] = column_max(max3_abs(12.f * inv[nv] * x, y, 0.f));
+      for (int i = 0; i < 16; i += 2) y = max3_abs(y, v[i >> 2][i & 3], v[i >> 2][(i & 3) + 1]);
+      bound = column_max(max3_abs(12.f * inv * x, y, 0.f));
     };
-    int first[NV];
-    bool any_bad = bad_token < C;
-#pragma unroll
-    for (int nv = 0; nv < NV; ++nv) {
-      first[nv] = C;
-      largest(nv);
-      any_bad |= __any(!finite(bound[nv]));
-    }
+    largest();
+    first = C;
+    any_bad = bad_token < C || __any(!finite(bound));
     if (any_bad) {
+      float at = C;
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) {
-        float at = C;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float& x = v[nv][i >> 2][i & 3];
-          if (!finite(x)) at = fminf(at, (float)(16 * (i >> 2) + 4 * grp + (i & 3))), x = 0.f;
-        }
-#pragma unroll
-        for (int kt = 0; kt < 8; ++kt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (!finite(S[nv][kt][j])) S[nv][kt][j] = 0.f, at = 0.f;
-        first[nv] = min(C - (int)column_max(C - at), bad_token);
-        largest(nv);
+      for (int i = 0; i < 16; ++i) {
+        float& x = v[i >> 2][i & 3];
+        if (!finite(x)) at = fminf(at, (float)(16 * (i >> 2) + 4 * grp + (i & 3))), x = 0.f;
       }
+#pragma unroll
+      for (int kt = 0; kt < 8; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!finite(S[kt][j])) S[kt][j] = 0.f, at = 0.f;
+      first = min(C - (int)column_max(C - at), bad_token);
+      largest();
     }
     // Each row's power of two puts 64 times its bound between 2^9 and 2^15. It
     // stays what it was while it does: then nothing is rescaled.
-    bool same = true;
-    float ratio[NV];
-#pragma unroll
-    for (int nv = 0; nv < NV; ++nv) {
-      const uint32_t ex = min(max((__float_as_uint(bound[nv]) >> 23) + 7, 21u), 254u);
-      const float scaled = bound[nv] * sc[nv];
-      ratio[nv] = 1.f;
-      if (!(scaled < 0x1p8f && scaled >= 0x1p2f)) {
-        const float s_new = __uint_as_float((268u - ex) << 23);
-        ratio[nv] = fminf(s_new * inv[nv], 0x1p126f);
-        sc[nv] = s_new, inv[nv] = __uint_as_float((ex - 14u) << 23);
-      }
-      same &= ratio[nv] == 1.f;
+    float ratio = 1.f;
+    const float scaled = bound * sc;
+    if (!(scaled < 0x1p8f && scaled >= 0x1p2f)) {
+      const uint32_t ex = min(max((__float_as_uint(bound) >> 23) + 7, 21u), 254u);
+      const float s_new = __uint_as_float((268u - ex) << 23);
+      ratio = fminf(s_new * inv, 0x1p126f);
+      sc = s_new, inv = __uint_as_float((ex - 14u) << 23);
     }
-    if (!__all(same)) {
+    if (__any(ratio != 1.f)) {
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-#pragma unroll
-        for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= ratio[nv];
+      for (int kt = 0; kt < 8; ++kt) S[kt] *= ratio;
     }
-    Operand<SPLIT> bs[NV][4];
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) bs[nv][s] = operand<SPLIT>(S[nv][2 * s], S[nv][2 * s + 1]);
+    for (int s = 0; s < 4; ++s) bs[s] = operand<SPLIT>(S[2 * s], S[2 * s + 1]);
 
-    // The products. Their LDS operands are read a stage or more before they
-    // are used, which the fences keep the compiler from undoing: a read just
-    // before its product costs its latency some 60 times a chunk.
-    f32x4_t u[NV][4], o[NV][4];
-    auto by_state = [&](int plane, f32x4_t(&x)[NV][4]) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        if (s + AHEAD < 4) read_rows(plane, s + AHEAD);
-        GDNR_COMPILER_FENCE();
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-          for (int nv = 0; nv < NV; ++nv)
-            x[nv][tt] = product<SPLIT>(f[s % (AHEAD + 1)][tt], bs[nv][s], s == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : x[nv][tt]);
-      }
-    };
-    by_state(0, u);  // K S0^T (its first fragments were read at the top)
+    f32x4_t u[4];
+    by_state(b, u);  // K S0^T
     GDNR_COMPILER_FENCE();
-    Operand<SPLIT> tf[kTri];
-    auto read_triangle = [&](int base) {
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int s = 0; s <= tt / 2; ++s) tf[tri(tt, s)] = triangle(base, tt, s);
-    };
-    f32x4_t be[4], bg[4];
+    f32x4_t be[4], bg[4], ed[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) be[tt] = beta4[4 * tt + grp], bg[tt] = held4[4 * tt + grp];
-    if constexpr (!SPLIT) read_triangle(0);
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) read_rows(P, s);
+    if constexpr (!SPLIT) read_triangle(tiles);
     GDNR_COMPILER_FENCE();
     // R = beta (v - e^G (K S0^T))
-    Operand<SPLIT> ub[NV][2], ud[NV][2];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
+      for (int j = 0; j < 4; ++j) u[tt][j] = fmaf(bg[tt][j], u[tt][j], be[tt][j] * (v[tt][j] * sc));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[nv][tt][j] = fmaf(bg[tt][j], u[nv][tt][j], be[tt][j] * (v[nv][tt][j] * sc[nv]));
-#pragma unroll
-    for (int nv = 0; nv < NV; ++nv)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) ub[nv][s] = operand<SPLIT>(u[nv][2 * s], u[nv][2 * s + 1]);
-    // U = R + (T - I) R
-    if constexpr (SPLIT) {
-      read_triangle(0);
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) u[nv][tt] *= kUp;
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int tt = 2 * s; tt < 4; ++tt)
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) u[nv][tt] = product<SPLIT>(tf[tri(tt, s)], ub[nv][s], u[nv][tt]);
-    by_state(P, o);  // Q S0^T
-    GDNR_COMPILER_FENCE();
-    f32x4_t ed[4];
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) ed[tt] = end4[4 * tt + grp];
+    for (int s = 0; s < 2; ++s) ub[s] = operand<SPLIT>(u[2 * s], u[2 * s + 1]);
     constexpr int KT = SPLIT ? 2 : 4;  // tiles of the keys read ahead
     Operand<SPLIT> kf[2][KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) kf[0][kt] = turned(kt, 0);
-    if constexpr (!SPLIT) read_triangle(kTri);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) ed[tt] = end4[4 * tt + grp];
     GDNR_COMPILER_FENCE();
+    // U = R + (T - I) R
+    if constexpr (SPLIT) {
+      read_triangle(tiles);
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv) {
-      if constexpr (SPLIT) {
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) u[nv][tt] *= kDown;
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        ud[nv][s] = operand<SPLIT>(u[nv][2 * s] * ed[2 * s], u[nv][2 * s + 1] * ed[2 * s + 1]);
-        ub[nv][s] = operand<SPLIT>(u[nv][2 * s], u[nv][2 * s + 1]);
-      }
+      for (int tt = 0; tt < 4; ++tt) u[tt] *= kUp;
     }
-    // the state after the chunk
+    by_triangle(u);
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv)
+    for (int kt = 0; kt < 8; ++kt) S[kt] *= total * kUp;
+    Operand<SPLIT> ud[2];
+    if constexpr (SPLIT) {
 #pragma unroll
-      for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= total * kUp;
+      for (int tt = 0; tt < 4; ++tt) u[tt] *= kDown;
+    }
 #pragma unroll
-    for (int i = 0; i < 16 / KT; ++i) {  // KT tiles of one half of the tokens at a time
+    for (int s = 0; s < 2; ++s) {
+      ud[s] = operand<SPLIT>(u[2 * s] * ed[2 * s], u[2 * s + 1] * ed[2 * s + 1]);
+      ub[s] = operand<SPLIT>(u[2 * s], u[2 * s + 1]);
+    }
+    // the state after the chunk, KT tiles of one half of the tokens at a time
+#pragma unroll
+    for (int i = 0; i < 16 / KT; ++i) {
       if (i + 1 < 16 / KT) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) kf[(i + 1) & 1][kt] = turned(((i + 1) * KT + kt) % 8, (i + 1) * KT / 8);
       }
       GDNR_COMPILER_FENCE();
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) {
-          f32x4_t& x = S[nv][(i * KT + kt) % 8];
-          x = product<SPLIT>(kf[i & 1][kt], ud[nv][i * KT / 8], x);
-        }
+      for (int kt = 0; kt < KT; ++kt) {
+        f32x4_t& x = S[(i * KT + kt) % 8];
+        x = product<SPLIT>(kf[i & 1][kt], ud[i * KT / 8], x);
+      }
     }
     if constexpr (SPLIT) {
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-#pragma unroll
-        for (int kt = 0; kt < 8; ++kt) S[nv][kt] *= kDown;
+      for (int kt = 0; kt < 8; ++kt) S[kt] *= kDown;
     }
-    // the outputs
-    if constexpr (SPLIT) read_triangle(kTri);
-    f32x4_t gr[4];
+    if (any_bad && first < C) {
+#pragma unroll
+      for (int kt = 0; kt < 8; ++kt) S[kt] = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+    }
+  };
+
+  // the outputs of chunk c from bs, ub, inv, first and any_bad
+  auto output_step = [&](int c) {
+    const uint8_t* b = lds + queries_at(c);
+    const float* scal = (const float*)(ROLES ? b + plane_bytes(SPLIT) + tri_bytes(SPLIT) : lds + (c & 1) * L::KEYS + plane_bytes(SPLIT));
+    const f32x4_t* grow4 = (const f32x4_t*)(scal + 3 * C);
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) read_rows(b, s);
+    f32x4_t o[4], gr[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) gr[tt] = grow4[4 * tt + grp];
+    GDNR_COMPILER_FENCE();
+    if constexpr (!SPLIT) read_triangle(b + plane_bytes(SPLIT));
+    by_state(b, o);  // Q S0^T
+    if constexpr (SPLIT) read_triangle(b + plane_bytes(SPLIT));
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
+    for (int tt = 0; tt < 4; ++tt) o[tt] *= gr[tt];
+    by_triangle(o);
+    const float scale = kDown * a.out_scale * inv;
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) o[nv][tt] *= gr[tt];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int tt = 2 * s; tt < 4; ++tt)
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) o[nv][tt] = product<SPLIT>(tf[tri(tt, s)], ub[nv][s], o[nv][tt]);
-#pragma unroll
-    for (int nv = 0; nv < NV; ++nv) {
-      const float f = kDown * a.out_scale * inv[nv];
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) o[nv][tt] *= f;
-    }
+    for (int tt = 0; tt < 4; ++tt) o[tt] *= scale;
     if (any_bad) {
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (16 * (i >> 2) + 4 * grp + (i & 3) >= first[nv]) o[nv][i >> 2][i & 3] = __builtin_nanf("");
-        if (first[nv] < C) {
-#pragma unroll
-          for (int kt = 0; kt < 8; ++kt) S[nv][kt] = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
-        }
-      }
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i >> 2) + 4 * grp + (i & 3) >= first) o[i >> 2][i & 3] = __builtin_nanf("");
     }
-    // (the next chunk's operands are waited for before the stores, which then
+    // (what is on its way to LDS is waited for before the stores, which then
     // have a whole chunk to drain)
-    if (BUFS == 2) GDNR_WAIT_VMCNT(0);
+    GDNR_WAIT_VMCNT(0);
     uint8_t* orow = op + c * C * o_row;
-    auto store_o = [&](int i) {
-      uint8_t* p = orow + (16 * (i >> 2) + (i & 3)) * o_row + o_lane;
-      if constexpr (NV == 2) Act::st2(p, o[0][i >> 2][i & 3], o[1][i >> 2][i & 3]);
-      else Act::st(p, 0, o[0][i >> 2][i & 3]);
-    };
+    auto store = [&](int i) { Act::st(orow + (16 * (i >> 2) + (i & 3)) * o_row + o_lane, 0, o[i >> 2][i & 3]); };
     if ((c + 1) * C <= len) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) store_o(i);
+      for (int i = 0; i < 16; ++i) store(i);
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (c * C + 16 * (i >> 2) + (i & 3) + 4 * grp < len) store_o(i);
+        if (c * C + 16 * (i >> 2) + (i & 3) + 4 * grp < len) store(i);
     }
-    if (BUFS == 1 && c + 1 < chunks) {
+  };
+
+  if (chain) {
+#pragma unroll
+    for (int kt = 0; kt < 8; ++kt) {
+      Raw<St, 4> x;
+      if (started) x.load(sp + 16 * kt * St::kBytes);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[kt][j] = started ? x[j] : 0.f;
+    }
+    if (chunks) fetch_keys(0), fetch_v(0);
+    if (!ROLES && !SPLIT && chunks) fetch_queries(0);
+    GDNR_WAIT_VMCNT(0);
+  }
+  if constexpr (ROLES) {
+    for (int c = 0; c <= chunks; ++c) {
+      __syncthreads();  // chunk c - 1 is handed over; what it read may be overwritten
+      uint8_t* handed = lds + 2 * L::KEYS + L::QBUFS * L::QUERIES + 16 * lane;
+      if (chain && c < chunks) {
+        state_step(c);
+        u32x4_t* to = (u32x4_t*)(handed + (c & 1) * L::HANDED);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) to[64 * s] = bs[s].hi;
+        to[64 * 4] = ub[0].hi, to[64 * 5] = ub[1].hi;
+        to[64 * 6] = u32x4_t{__float_as_uint(inv), (uint32_t)first, any_bad, 0};
+        GDNR_WAIT_VMCNT(0);
+      }
+      if (outputs) {
+        if (c < chunks) fetch_queries(c);
+        if (c > 0) {
+          const u32x4_t* from = (const u32x4_t*)(handed + ((c - 1) & 1) * L::HANDED);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) bs[s].hi = from[64 * s];
+          ub[0].hi = from[64 * 4], ub[1].hi = from[64 * 5];
+          const u32x4_t x = from[64 * 6];
+          inv = __uint_as_float(x[0]), first = (int)x[1], any_bad = __builtin_amdgcn_readfirstlane(x[2]) != 0;
+          output_step(c - 1);
+        } else {
+          GDNR_WAIT_VMCNT(0);
+        }
+      }
+    }
+  } else {
+    for (int c = 0; c < chunks; ++c) {
+      // chunk c's operands are in LDS (every wave waited for its part), those of
+      // c - 1 are no longer read
       __syncthreads();
-      fetch(c + 1);
-      GDNR_WAIT_VMCNT(0);
+      if (!SPLIT && c + 1 < chunks) fetch_queries(c + 1);
+      state_step(c);
+      if constexpr (SPLIT) {  // the one buffer of queries was filled meanwhile
+        GDNR_WAIT_VMCNT(0);
+        __syncthreads();
+      }
+      output_step(c);
     }
   }
-#pragma unroll
-  for (int nv = 0; nv < NV; ++nv)
+  if (chain) {
 #pragma unroll
     for (int kt = 0; kt < 8; ++kt)
 #pragma unroll
-      for (int j = 0; j < 4; j += 2)
-        St::st2(sp + (nv * a.st_v + 16 * kt + j) * St::kBytes, S[nv][kt][j] * inv[nv], S[nv][kt][j + 1] * inv[nv]);
+      for (int j = 0; j < 4; j += 2) St::st2(sp + (16 * kt + j) * St::kBytes, S[kt][j] * inv, S[kt][j + 1] * inv);
+  }
 }
 
 // Whether results keep more than bf16 does.
@@ -944,23 +943,27 @@ int launch_prep(const PrefillArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((chunk_prep_kernel<Act, GATE_F32, SPLIT>), dim3(a.T / C + a.N, a.H), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
-template <class Act, class St, bool SPLIT, int WAVES, int NV>
+template <class Act, class St, bool SPLIT, int WAVES, bool ROLES>
 int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
-  constexpr int lds = scan_buffers(SPLIT) * (2 * (SPLIT ? 2 : 1) * C * 2 * K + (int)head_bytes(SPLIT));
+  constexpr int lds = ScanLds<SPLIT, ROLES>::BYTES;
   static_assert(lds <= kMaxStepLds, "the operands fit");
-  const auto kernel = chunk_scan_kernel<Act, St, SPLIT, WAVES, NV>;
+  const auto kernel = chunk_scan_kernel<Act, St, SPLIT, WAVES, ROLES>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(kernel, dim3(a.HV * (a.V / (16 * NV * WAVES)), a.N), dim3(64 * WAVES), lds, s, a);
+  hipLaunchKernelGGL(kernel, dim3(a.HV * (a.V / (ROLES ? 16 : 16 * WAVES)), a.N), dim3(64 * WAVES), lds, s, a);
   return (int)hipGetLastError();
 }
+// A workgroup's LDS leaves room for one on a compute unit. While workgroups of
+// all of a head's V-rows (or half of them) would fill the card, those share its
+// operands; otherwise the chain over a sequence's chunks is what takes the
+// time, and it is spread as thin as it goes.
 template <class Act, class St, bool SPLIT>
 int launch_scan(const PrefillArgs& a, hipStream_t s) {
-  // all of a head's V-rows in one workgroup once that fills the card
   const int64_t heads = (int64_t)a.N * a.HV;
-  if (a.V % 128 == 0 && heads * (a.V / 128) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 8, 1>(a, s);
-  if (a.V % 64 == 0 && heads * (a.V / 64) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 4, 1>(a, s);
-  return launch_scan_as<Act, St, SPLIT, 2, 1>(a, s);
+  if (a.V % 128 == 0 && heads * (a.V / 128) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 8, false>(a, s);
+  if (a.V % 64 == 0 && heads * (a.V / 64) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 4, false>(a, s);
+  if constexpr (SPLIT) return launch_scan_as<Act, St, SPLIT, 2, false>(a, s);
+  else return launch_scan_as<Act, St, SPLIT, 2, true>(a, s);
 }
 
 template <class Act, class St, bool GATE_F32>
