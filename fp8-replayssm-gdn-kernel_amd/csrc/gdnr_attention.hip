@@ -228,11 +228,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
     }
   };
   auto copy_values = [&]() {
+    uint32_t vr[NV];
+    int sub = lane / PPR;
+    asm volatile("" : "+v"(sub));  // (places formed here, not kept)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int r = i * RPI + lane / PPR;
-      dma16(vbase + (uint64_t)((uint32_t)__shfl((int)v_row, r) + (uint64_t)((lane % PPR) ^ row_key<D>(r))) * 16, vt_lds + i * 1024);
-    }
+    for (int i = 0; i < NV; ++i) vr[i] = (uint32_t)__shfl((int)v_row, i * RPI + sub);
+    GDNR_COMPILER_FENCE();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      dma16(vbase + (vr[i] + (uint64_t)((lane % PPR) ^ row_key<D>(i * RPI + sub))) * 16, vt_lds + i * 1024);
   };
 
   f32x4_t o[DT];
@@ -378,7 +382,7 @@ template <int D>
 struct Tile {
   static constexpr int NT = D == 256 ? 1 : 2;      // 16-row tiles a wave
   static constexpr int ROWS = kWaves * NT * 16;    // rows a workgroup
-  static constexpr int KEYS = D == 256 ? 32 : 64;  // keys a step
+  static constexpr int KEYS = 8192 / D;            // keys a step
   static constexpr int KB = KEYS * 2 * D;          // bytes of a step's keys (and of its values)
   static constexpr int LDS = 4 * KB;               // two steps' keys and values
 };

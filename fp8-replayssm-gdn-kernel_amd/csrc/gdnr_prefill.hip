@@ -108,19 +108,24 @@ __global__ __launch_bounds__(256) void recurrent_kernel(const PrefillArgs a) {
   const float a_log = a.a_log[hv * a.al_s], dt_bias = a.dt_bias[hv * a.db_s];
   Raw<Act, 8> q, k, qn, kn;
   Raw<Act, 4> v, vn;
-  float ag, bg, agn, bgn;
   auto fetch = [&](int t) {
     const uint8_t* row = (const uint8_t*)a.mixed + (int64_t)t * a.mx_t * ES;
     qn.load(row + (h * K + 8 * cl) * ES);
     kn.load(row + ((a.H + h) * K + 8 * cl) * ES);
     vn.load(row + (2 * a.H * K + hv * a.V + row0 + 4 * grp) * ES);
-    agn = Gate::ld(a.a, (int64_t)t * a.a_t + hv * a.a_h);
-    bgn = Gate::ld(a.bgate, (int64_t)t * a.bg_t + hv * a.bg_h);
+  };
+  // the gates of 64 tokens at once, a lane a token
+  float gamma64 = 0.f, beta64 = 0.f;
+  auto gates = [&](int t) {
+    const int64_t at = min(t + lane, end - 1);
+    gamma64 = expf(log_decay(Gate::ld(a.a, at * a.a_t + hv * a.a_h) + dt_bias, a_log));
+    beta64 = sigmoid(Gate::ld(a.bgate, at * a.bg_t + hv * a.bg_h));
   };
   if (begin < end) fetch(begin);
   for (int t = begin; t < end; ++t) {
-    q = qn, k = kn, v = vn, ag = agn, bg = bgn;
+    q = qn, k = kn, v = vn;
     if (t + 1 < end) fetch(t + 1);
+    if (((t - begin) & 63) == 0) gates(t);
     float qf[8], kf[8], qq = 0.f, kk = 0.f, qk = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -129,8 +134,8 @@ __global__ __launch_bounds__(256) void recurrent_kernel(const PrefillArgs a) {
       kk = fmaf(kf[e], kf[e], kk);
       qk = fmaf(qf[e], kf[e], qk);
     }
-    const float rq = 1.f / sqrtf(sum16(qq) + 1e-6f), rk = 1.f / sqrtf(sum16(kk) + 1e-6f);
-    const float gamma = expf(log_decay(ag + dt_bias, a_log)), beta = sigmoid(bg);
+    const float rq = __builtin_amdgcn_rsqf(sum16(qq) + 1e-6f), rk = __builtin_amdgcn_rsqf(sum16(kk) + 1e-6f);
+    const float gamma = readlane_f(gamma64, (t - begin) & 63), beta = readlane_f(beta64, (t - begin) & 63);
     qk = sum16(qk) * rq * rk;
     float o[4];
 #pragma unroll
