@@ -940,8 +940,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 // Whether results keep more than bf16 does.
 bool needs_split(int act_dt, int state_dt) { return act_dt != DT_BF16 || state_dt != DT_BF16; }
 
-// The chunked form from an average of 16 tokens a sequence on.
-bool chunked_form(int64_t T, int64_t N) { return T >= 16 * N; }
+// The chunked form from an average of 16 tokens a sequence on (SPLIT: 32). us
+// a call, token by token and in chunks, HV=32, V=128, bf16: one sequence of 16
+// tokens 14.9 and 19.5, of 24 20.0 and 19.4; 64 sequences of 8 72 and 109, of 16
+// 125 and 110; f16 with an f32 state, 4 sequences of 32 25.6 and 29.0, of 64 46
+// and 29.
+bool chunked_form(int64_t T, int64_t N, bool split) { return T >= (split ? 32 : 16) * N; }
 
 template <class Act, bool GATE_F32, bool SPLIT>
 int launch_prep(const PrefillArgs& a, hipStream_t s) {
@@ -958,17 +962,24 @@ int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(kernel, dim3(a.HV * (a.V / (ROLES ? 16 : 16 * WAVES)), a.N), dim3(64 * WAVES), lds, s, a);
   return (int)hipGetLastError();
 }
-// A workgroup's LDS leaves room for one on a compute unit. While workgroups of
-// all of a head's V-rows (or half of them) would fill the card, those share its
-// operands; otherwise the chain over a sequence's chunks is what takes the
-// time, and it is spread as thin as it goes.
+// A workgroup's LDS leaves room for one on a compute unit, so the scan's time is
+// the rounds its workgroups take over the card times what a chunk costs them:
+// with 8 waves (128 V-rows) 3.7 us, 4 waves 2.8, one and its outputs' wave
+// (16 V-rows) 2.0; with SPLIT operands 7.0 and 5.0, and with 2 waves (32
+// V-rows) 4.7. The cheapest product runs, the wider one of equals (it reads the
+// operands once for more rows). us a call of 1024 tokens a sequence, HV=32,
+// V=128, with 8 waves, 4 and the pair: 2 sequences 81, 65 and 77; 4: 91, 79 and
+// 136; 6: 113, 133 and 202; 8: 128, 144 and 266.
 template <class Act, class St, bool SPLIT>
 int launch_scan(const PrefillArgs& a, hipStream_t s) {
-  const int64_t heads = (int64_t)a.N * a.HV;
-  if (a.V % 128 == 0 && heads * (a.V / 128) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 8, false>(a, s);
-  if (a.V % 64 == 0 && heads * (a.V / 64) >= device_cus()) return launch_scan_as<Act, St, SPLIT, 4, false>(a, s);
-  if constexpr (SPLIT) return launch_scan_as<Act, St, SPLIT, 2, false>(a, s);
-  else return launch_scan_as<Act, St, SPLIT, 2, true>(a, s);
+  const int64_t rows = (int64_t)a.N * a.HV * a.V, cus = device_cus();
+  const auto cost = [&](int columns, int chunk) {
+    return a.V % columns ? INT64_MAX : (rows / columns + cus - 1) / cus * chunk;
+  };
+  const int64_t eight = cost(128, SPLIT ? 70 : 37), four = cost(64, SPLIT ? 50 : 28), thin = cost(SPLIT ? 32 : 16, SPLIT ? 47 : 20);
+  if (eight <= four && eight <= thin) return launch_scan_as<Act, St, SPLIT, 8, false>(a, s);
+  if (four <= thin) return launch_scan_as<Act, St, SPLIT, 4, false>(a, s);
+  return launch_scan_as<Act, St, SPLIT, 2, !SPLIT>(a, s);
 }
 
 template <class Act, class St, bool GATE_F32>
@@ -980,7 +991,8 @@ int launch_recurrent(const PrefillArgs& a, hipStream_t s) {
 
 template <class Act, bool GATE_F32>
 int launch_state(const PrefillArgs& a, int state_dt, hipStream_t s) {
-  if (chunked_form(a.T, a.N)) {
+  constexpr int ACT = std::is_same<Act, ActBF16>::value ? DT_BF16 : std::is_same<Act, ActF16>::value ? DT_F16 : DT_F32;
+  if (chunked_form(a.T, a.N, needs_split(ACT, state_dt))) {
     if constexpr (std::is_same<Act, ActBF16>::value) {
       if (state_dt == DT_BF16) {
         const int rc = launch_prep<Act, GATE_F32, false>(a, s);
@@ -1001,8 +1013,8 @@ int launch_state(const PrefillArgs& a, int state_dt, hipStream_t s) {
 }  // namespace
 
 int64_t prefill_work_bytes(int64_t T, int64_t N, int32_t H, int32_t HV, int act_dt, int state_dt) {
-  if (!chunked_form(T, N)) return 0;
   const bool split = needs_split(act_dt, state_dt);
+  if (!chunked_form(T, N, split)) return 0;
   return (T / C + N) * (H * unit_bytes(split) + HV * head_bytes(split));
 }
 
