@@ -275,13 +275,37 @@ __host__ __device__ constexpr int unit_at(int t, int k4) {
 // index of the tile (16 rows of t, 32 columns of i) in a lower triangle
 __host__ __device__ constexpr int tri(int tt, int ts) { return tt < 2 ? tt : 2 * (tt - 1) + ts; }
 
-// 2^d of a difference of sums of log2 decays; SPLIT: with what rounding the
-// exponent to f32 leaves out
+// A sum of log2 decays as two floats, hi the rounded sum and lo what that leaves.
+// 2^(a - b): the difference of the hi's is off by 2^-24 of itself at most, which
+// SPLIT corrects along with the lo's.
 template <bool SPLIT>
-__device__ __forceinline__ float exp2_diff(double d) {
-  const float h = (float)d, e = __builtin_amdgcn_exp2f(h);
-  if constexpr (!SPLIT) return e;
-  return fmaf(e, 0.6931471805599453f * (float)(d - (double)h), e);
+__device__ __forceinline__ float exp2_diff(float2 a, float2 b) {
+  const float d = a.x - b.x, e = __builtin_amdgcn_exp2f(d);
+  const float t = d - a.x;  // (two-sum: what a.x - b.x rounded off)
+  const float rest = (SPLIT ? (a.x - (d - t)) - (b.x + t) : 0.f) + (a.y - b.y);
+  return fmaf(e, 0.6931471805599453f * rest, e);
+}
+__device__ __forceinline__ double readlane_d(double x, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double x) {  // lanes with no source get 0
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, (uint64_t)dpp_u<CTRL>((uint32_t)(b >> 32)) << 32 | dpp_u<CTRL>((uint32_t)b));
+}
+// sum over the lanes up to this one, and over all 64: within rows of 16 lanes,
+// then the rows before
+__device__ __forceinline__ double prefix_sum(double x, double& total) {
+  x += dpp_d<0x111>(x);
+  x += dpp_d<0x112>(x);
+  x += dpp_d<0x114>(x);
+  x += dpp_d<0x118>(x);
+  const double r0 = readlane_d(x, 15), r1 = r0 + readlane_d(x, 31), r2 = r1 + readlane_d(x, 47);
+  total = r2 + readlane_d(x, 63);
+  const int row = (threadIdx.x & 63) >> 4;
+  return x + (row == 0 ? 0.0 : row == 1 ? r0 : row == 2 ? r1 : r2);
 }
 
 // One chunk of one key head: 4 waves. The Gram products are formed transposed
@@ -293,7 +317,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
   constexpr int ES = Act::kBytes, RS = 2 * K + 16, P = SPLIT ? 2 : 1;  // LDS row of a key or query, halves
   constexpr int kUnits = 2 * P * C * RS, MS = 68 * 4, kM = C * MS;      // [i][t] f32 of M, per head
   __shared__ __attribute__((aligned(16))) uint8_t lds[kUnits > 2 * kM ? kUnits : 2 * kM];
-  __shared__ double Gs[2][C];  // sums of log2 decays
+  __shared__ float2 Gs[2][C];  // sums of log2 decays
   __shared__ float betas[2][C];
   __shared__ int bad_key;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -341,7 +365,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = t < len ? rows[i][e] : 0.f, ss = fmaf(x[e], x[e], ss);
     ss = sum16(ss);
-    float f = 1.f / sqrtf(ss + 1e-6f);
+    float f = __builtin_amdgcn_rsqf(ss + 1e-6f);
     if (!is_q && !(ss < __builtin_inff())) {
       if (col == 0) atomicMin(&bad_key, t);
       f = 0.f;
@@ -401,41 +425,43 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
       const int first = bads ? __ffsll((unsigned long long)bads) - 1 : C;
       if (t >= first) g = 0.f, beta = 0.f;
       // (a decay of e^-1e4 is 0 in every format; a sum of such stays exact)
-      double G = (double)fmaxf(g, -1e4f) * 1.4426950408889634;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const double up = __shfl_up(G, d);
-        if (lane >= d) G += up;
-      }
-      const double last = __shfl(G, 63);
+      double last;
+      const double sum = prefix_sum((double)fmaxf(g, -1e4f) * 1.4426950408889634, last);
+      const float2 G = make_float2((float)sum, (float)(sum - (double)(float)sum));
+      const float2 end = make_float2((float)last, (float)(last - (double)(float)last));
       Gs[wave][t] = G;
       betas[wave][t] = beta;
       float* sc = (float*)(w.head + ((int64_t)slot * a.HV + hv) * head_bytes(SPLIT));
-      const float grow = exp2_diff<SPLIT>(G);
+      const float grow = exp2_diff<SPLIT>(G, make_float2(0.f, 0.f));
       sc[t] = beta;
       sc[C + t] = -beta * grow * (SPLIT ? 1.f / kFix : 1.f);
-      sc[2 * C + t] = exp2_diff<SPLIT>(last - G);
+      sc[2 * C + t] = exp2_diff<SPLIT>(end, G);
       sc[3 * C + t] = grow;
       if (t == 0) ((int*)sc)[4 * C] = first;
     }
     __syncthreads();
+#pragma nounroll
     for (int e = 0; e < heads; ++e) {
       uint8_t* tiles = w.head + ((int64_t)slot * a.HV + h * a.G + g0 + e) * head_bytes(SPLIT) + kScalars;
       const int t = 16 * wave + col;
-      const double Gt = Gs[e][t];
+      const float2 Gt = Gs[e][t];
       const float bt = betas[e][t];
       f32x4_t at[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         at[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         if (c > wave) continue;
+        f32x4_t m;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 16 * c + 4 * grp + j;
-          const float decay = i <= t ? exp2_diff<SPLIT>(Gt - Gs[e][i]) : 0.f;
+          const float2 Gi = Gs[e][i];
+          const float decay = exp2_diff<SPLIT>(i <= t ? Gt : Gi, Gi);
           at[c][j] = i <= t ? decay * qk[c][j] : 0.f;
-          *(float*)(lds + e * kM + i * MS + t * 4) = i < t ? bt * decay * kk[c][j] : 0.f;
+          m[j] = i < t ? bt * decay * kk[c][j] : 0.f;
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(float*)(lds + e * kM + (16 * c + 4 * grp + j) * MS + t * 4) = m[j];
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -448,30 +474,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
     }
     __syncthreads();
     // T = (I + M)^-1 by blocks of 16, wave w the block row w. First its
-    // diagonal block, a lane a row of it (lanes of group e: head g0 + e): from
-    // x (I + M) = e_t, the last column first. It takes M's place.
+    // diagonal block, a lane a column of it (lanes of group e: head g0 + e): (I + M) x
+    // = e_c, each entry, once known, taken out of all below it. It takes M's place.
     if (grp < heads) {
-      uint8_t* m = lds + grp * kM + 16 * wave * (MS + 4);
+      uint8_t* m = lds + grp * kM + 16 * wave * (MS + 4);  // [i][t]
       float x[16];
 #pragma unroll
-      for (int i = 15; i >= 0; --i) {
-        x[i] = col == i ? 1.f : 0.f;
+      for (int t = 0; t < 16; ++t) x[t] = col == t ? 1.f : 0.f;
 #pragma unroll
-        for (int q = 3; q >= (i + 1) / 4; --q) {
-          const f32x4_t row = *(const f32x4_t*)(m + i * MS + 16 * q);
+      for (int i = 0; i < 15; ++i)
 #pragma unroll
-          for (int j = 3; j >= 0; --j)
-            if (4 * q + j > i) x[i] = fmaf(-x[4 * q + j], row[j], x[i]);
+        for (int q = (i + 1) / 4; q < 4; ++q) {
+          const f32x4_t mi = *(const f32x4_t*)(m + i * MS + 16 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (4 * q + j > i) x[4 * q + j] = fmaf(-x[i], mi[j], x[4 * q + j]);
         }
-      }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) *(float*)(m + i * MS + 4 * col) = x[i];
+      for (int q = 0; q < 4; ++q) *(f32x4_t*)(m + col * MS + 16 * q) = f32x4_t{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
     }
     __syncthreads();
     // Then T_wJ = -(sum over L = J+1..w of T_wL M_LJ) T_JJ, the nearest block
     // first, transposed (rows of J on registers, t on lanes): what one product
     // leaves is the next one's right operand, and M and T_JJ are read from LDS
     // as they lie.
+#pragma nounroll
     for (int e = 0; e < heads; ++e) {
       const uint8_t* m = lds + e * kM;
       f32x4_t x[4];
@@ -482,6 +509,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[c][j] = *(const float*)(m + (16 * c + 4 * grp + j) * MS + (16 * c + col) * 4);
         if (c >= wave) continue;
+        const f32x4_t tl = *(const f32x4_t*)(m + (16 * c + col) * MS + (16 * c + 4 * grp) * 4);
         f32x4_t y = x[c];
 #pragma unroll
         for (int l = c + 1; l < 4; ++l) {
@@ -490,7 +518,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
 #pragma unroll
           for (int j = 0; j < 4; ++j) y = __builtin_amdgcn_mfma_f32_16x16x4f32(ml[j], x[l][j], y, 0, 0, 0);
         }
-        const f32x4_t tl = *(const f32x4_t*)(m + (16 * c + col) * MS + (16 * c + 4 * grp) * 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(-tl[j], y[j], x[c], 0, 0, 0);
       }
