@@ -53,6 +53,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   Act::st2(&w, lo, hi);
   return w;
 }
+// 16 x 32 ones: their product with rounded weights is the weights' sum, in every
+// row of the result
+template <class Act>
+__device__ __forceinline__ u32x4_t ones() {
+  constexpr uint32_t kOne = std::is_same<Act, ActBF16>::value ? 0x3F803F80u : 0x3C003C00u;
+  return u32x4_t{kOne, kOne, kOne, kOne};
+}
 // 4 rows (keys) x 16 columns at p (row stride in bytes), transposed: lane i of
 // each 16-lane group receives column i of the group's 4 rows
 __device__ __forceinline__ uint2 transposed4(const uint8_t* p) {
@@ -75,14 +82,7 @@ __device__ __forceinline__ float column_max(float x) {
   const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
   return fmaxf(__uint_as_float(row[0]), __uint_as_float(row[1]));
 }
-__device__ __forceinline__ float column_sum(float x) {
-  const uint32_t b = __float_as_uint(x);
-  const auto half = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  const uint32_t h = __float_as_uint(__uint_as_float(half[0]) + __uint_as_float(half[1]));
-  const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
-  return __uint_as_float(row[0]) + __uint_as_float(row[1]);
-}
-// x *= f and x += a b in the registers where x lies: of the two sides of a
+// x *= f, x += d and x += a b in the registers where x lies: of the two sides of a
 // branch, the one that leaves x alone then has nothing to copy
 __device__ __forceinline__ void scale_in_place(f32x4_t& x, float f) {
 #pragma unroll
@@ -242,7 +242,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
   f32x4_t o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m_run = -__builtin_inff(), l_run = 0.f;
+  float m_run = -__builtin_inff();
+  f32x4_t l_run = {0.f, 0.f, 0.f, 0.f};  // (every row of it)
   constexpr int STEP = kWaves * kKeys;
   int key0 = k_begin + wave * kKeys;
   if (key0 < k_end) {
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
     if (__any(top > m_run)) {
       const float m_new = fmaxf(m_run, top);
       const float f = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-      l_run *= f;
+      scale_in_place(l_run, f);
 #pragma unroll
       for (int i = 0; i < DT; ++i) scale_in_place(o[i], f);
       m_run = m_new;
@@ -284,7 +285,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
     const float base = m_run == -__builtin_inff() ? 0.f : m_run;
     float p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - base), l_run += p[e];
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - base);
     bool bad = false;
     if constexpr (MASKED) {
 #pragma nounroll
@@ -301,6 +302,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
             if (4 * (key >> 4) + (key & 3) == e) pk = p[e];
           pk = __shfl(pk, col + 16 * ((key >> 2) & 3));
           const uint32_t seen = key0 + key < vis ? ~0u : 0u;
+          shift_in_place(l_run, pk);
 #pragma unroll
           for (int i = 0; i < DT; ++i) {
             const uint2 w = *(const uint2*)(vt + key * 2 * D + 16 * ((2 * i + (grp >> 1)) ^ row_key<D>(key)) + 8 * (grp & 1));
@@ -311,9 +313,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
       }
     }
     if (!bad) {
-      // (the sum is of the unrounded weights; rounding them to the cache's type
-      // costs the output about its own rounding)
+      // (the weights are rounded to the cache's type, which costs the output
+      // about its own rounding; their sum is of the rounded ones, so that a row
+      // that one key rules loses nothing)
       const u32x4_t pf = {pack2<Act>(p[0], p[1]), pack2<Act>(p[2], p[3]), pack2<Act>(p[4], p[5]), pack2<Act>(p[6], p[7])};
+      l_run = mfma<Act>(ones<Act>(), pf, l_run);
       uint32_t v_key = row_key<D>(4 * grp + (col >> 2)) ^ ((col & 3) >> 1);
       asm volatile("" : "+v"(v_key));  // (addresses formed here, not kept)
       const uint8_t* vl = vt + (4 * grp + (col >> 2)) * 2 * D + 8 * (col & 1);
@@ -336,15 +340,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
   };
   for (; key0 + kKeys <= vis_all; key0 += STEP) step(std::false_type{});
   for (; key0 < k_end; key0 += STEP) step(std::true_type{});
-  l_run = column_sum(l_run);
-
   // join the waves: every row's sums at the largest maximum
   __syncthreads();
   float* ml = (float*)(lds + lds_bytes<D>() - kWaves * kRows * 8);
   uint8_t* ow = lds + wave * kRows * o_stride<D>() + col * o_stride<D>() + 16 * grp;
 #pragma unroll
   for (int i = 0; i < DT; ++i) *(f32x4_t*)(ow + 64 * i) = o[i];
-  if (grp == 0) ml[2 * (wave * kRows + col)] = m_run, ml[2 * (wave * kRows + col) + 1] = l_run;
+  if (grp == 0) ml[2 * (wave * kRows + col)] = m_run, ml[2 * (wave * kRows + col) + 1] = l_run[0];
   __syncthreads();
   const int row = threadIdx.x >> 4, dl = threadIdx.x & 15;
   const int t = tok0 + row / gt, head = ht * kRows + row % gt;
@@ -474,10 +476,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
 
   f32x4_t o[NT][DT];
-  float m_run[NT], l_run[NT];
+  f32x4_t l_run[NT];  // (every row of it)
+  float m_run[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m_run[nt] = -__builtin_inff(), l_run[nt] = 0.f;
+    m_run[nt] = -__builtin_inff(), l_run[nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[nt][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
@@ -579,7 +582,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int nt = 0; nt < NT; ++nt) {
         const float m_new = fmaxf(m_run[nt], top[nt] * scale);
         const float f = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m_run[nt] - m_new);
-        l_run[nt] *= f;
+        scale_in_place(l_run[nt], f);
 #pragma unroll
         for (int i = 0; i < DT; ++i) scale_in_place(o[nt][i], f);
         m_run[nt] = m_new;
@@ -595,15 +598,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int m = 0; m < MT; ++m) scale_in_place(s[m][nt], f), shift_in_place(s[m][nt], base);
         base = 0.f, f = 1.f;
       }
-      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[m][nt][j] = __builtin_amdgcn_exp2f(fmaf(s[m][nt][j], f, base));
-          sum[j & 1] += s[m][nt][j];
-        }
-      l_run[nt] += sum[0] + sum[1];
+        for (int j = 0; j < 4; ++j) s[m][nt][j] = __builtin_amdgcn_exp2f(fmaf(s[m][nt][j], f, base));
     }
     if constexpr (MASKED) {
       bool bad = false;
@@ -622,6 +620,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
               if (4 * (key >> 4) + (key & 3) == e) pk = s[e >> 2][nt][e & 3];
             pk = __shfl(pk, col + 16 * ((key >> 2) & 3));
             const uint32_t seen = key0 + key < vis[nt] ? ~0u : 0u;
+            shift_in_place(l_run[nt], pk);
 #pragma unroll
             for (int i = 0; i < DT; ++i) {
               const uint2 w = *(const uint2*)(vt + key * 2 * D + 16 * ((2 * i + (grp >> 1)) ^ row_key<D>(key)) + 8 * (grp & 1));
@@ -632,8 +631,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         return;
       }
     }
-    // O^T += V^T P^T. (The sum is of the unrounded weights; rounding them to
-    // the cache's type costs the output about its own rounding.)
+    // O^T += V^T P^T. (The weights are rounded to the cache's type, which costs
+    // the output about its own rounding; their sum is of the rounded ones, so
+    // that a row that one key rules loses nothing.)
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int half = 0; half < MT / 2; ++half) {
@@ -642,6 +642,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int nt = 0; nt < NT; ++nt) {
         const f32x4_t x = s[2 * half][nt], y = s[2 * half + 1][nt];
         pf[nt] = u32x4_t{pack2<Act>(x[0], x[1]), pack2<Act>(x[2], x[3]), pack2<Act>(y[0], y[1]), pack2<Act>(y[2], y[3])};
+        l_run[nt] = mfma<Act>(ones<Act>(), pf[nt], l_run[nt]);
       }
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -660,7 +661,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const float l = column_sum(l_run[nt]);
+    const float l = l_run[nt][0];
     if (!live[nt]) continue;
     const int qh = hk * a.G + rh[nt];
     if (pieces > 1) {
