@@ -10,12 +10,15 @@ nothing synchronises.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
+import numpy as np
 import torch
 
 import gdnr_lib
 from gdn_replayssm_fp8_kernel import _as_f32, _as_i32
 
-__all__ = ["rope_table", "qkv_norm_rope_append", "paged_attention"]
+__all__ = ["rope_table", "qkv_norm_rope_append", "paged_attention", "PagedBatch", "PagedKVCache"]
 
 _APPEND = gdnr_lib.ENTRY_IDS["gdnr_qkv_norm_rope_append"]
 _ATTENTION = gdnr_lib.ENTRY_IDS["gdnr_paged_attention"]
@@ -99,7 +102,9 @@ def paged_attention(
         raise ValueError("q must be [T, HQ, D], k_cache [pages, page_size, HKV, D] and block_table [N, width]")
     tokens, heads, dim = q.shape
     if max_context is None:
-        max_context = block_table.shape[1] * k_cache.shape[1]
+        max_context = min(block_table.shape[1] * k_cache.shape[1], 2 ** 31 - 1)
+    elif not 0 <= max_context < 2 ** 31:
+        raise ValueError(f"max_context {max_context} outside [0, 2^31)")
     if out is None:
         out = host.empty(q, (tokens, heads, dim))
     if workspace is None:
@@ -109,3 +114,81 @@ def paged_attention(
     host.call(_ATTENTION, (q, k_cache, v_cache, _as_i32(block_table), _as_i32(cu_seqlens), _as_i32(context_lens), out,
                            workspace), (int(max_context),), (dim ** -0.5 if scale is None else scale,), None)
     return out
+
+
+@dataclass
+class PagedBatch:
+    """Device metadata of one step of PagedKVCache sequences, shared by every
+    layer of the step."""
+
+    positions: torch.Tensor     # [T] i32: position of each new token in its sequence
+    slot_mapping: torch.Tensor  # [T] i32: its slot in the caches
+    block_table: torch.Tensor   # [N, width] i32
+    cu_seqlens: torch.Tensor    # [N + 1] i32
+    context_lens: torch.Tensor  # [N] i32, new tokens included
+    max_context: int
+
+
+class PagedKVCache:
+    """Keys and values of ``layers`` attention layers in pages of ``page_size``
+    tokens that sequences take as they grow. Which pages a sequence holds is
+    host state (as ReplaySSMCache keeps its ring fills), the same for every
+    layer; step() turns a batch into the metadata its layers' two operators
+    take."""
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, layers: int = 1,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if num_pages < 1 or page_size < 1 or layers < 1:
+            raise ValueError("num_pages, page_size and layers must be at least 1")
+        self.page_size, self.device = page_size, torch.device(device)
+        self.k = [torch.zeros(num_pages, page_size, kv_heads, head_dim, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.v = [torch.zeros_like(k) for k in self.k]
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages: dict = {}   # sequence -> its pages, in order
+        self._length: dict = {}  # sequence -> tokens it holds
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, sequence) -> int:
+        return self._length.get(sequence, 0)
+
+    def release(self, sequence) -> None:
+        """End a sequence: its pages are free."""
+        self._free.extend(reversed(self._pages.pop(sequence, [])))
+        self._length.pop(sequence, None)
+
+    def step(self, sequences, new_tokens) -> PagedBatch:
+        """Room for new_tokens[i] further tokens of each sequence (any hashable
+        names, distinct; a new name starts a sequence) and the metadata of
+        appending and attending them. Raises, with nothing taken, when the
+        pages do not suffice."""
+        new = [int(x) for x in new_tokens]
+        if len(new) != len(sequences) or min(new, default=0) < 0:
+            raise ValueError("new_tokens must hold a count of at least 0 for each sequence")
+        if len(set(sequences)) != len(sequences):
+            raise ValueError("a sequence appears twice in the batch")
+        lengths = [self.length(s) + x for s, x in zip(sequences, new)]
+        held = [-(-x // self.page_size) for x in lengths]
+        need = sum(h - len(self._pages.get(s, [])) for s, h in zip(sequences, held))
+        if need > len(self._free):
+            raise RuntimeError(f"{need} pages needed, {len(self._free)} free")
+        width = max(held, default=0)
+        table = np.zeros((len(new), max(width, 1)), dtype=np.int32)
+        positions, slots = [], []
+        for i, (s, x, total, h) in enumerate(zip(sequences, new, lengths, held)):
+            pages = self._pages.setdefault(s, [])
+            while len(pages) < h:
+                pages.append(self._free.pop())
+            self._length[s] = total
+            table[i, :h] = pages
+            at = np.arange(total - x, total)
+            positions.append(at)
+            slots.append(table[i, at // self.page_size].astype(np.int64) * self.page_size + at % self.page_size)
+        # one copy for all of it
+        parts = [np.concatenate(positions or [[]]), np.concatenate(slots or [[]]), np.concatenate([[0], np.cumsum(new)]),
+                 np.asarray(lengths), table.reshape(-1)]
+        packed = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(self.device)
+        pos, slot, cu, context, flat = packed.split([p.size for p in parts])
+        return PagedBatch(pos, slot, flat.view(table.shape), cu, context, max(lengths, default=0))

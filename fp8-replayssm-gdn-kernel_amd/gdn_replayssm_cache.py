@@ -19,7 +19,9 @@ ReplaySSMCache combines the two:
     ONE fused launch (gdn_prep_replay_fp8 with state_indices), and advances
     the fills: 0 after a flush (the ring restarts), fill + 1 otherwise.
     Padding entries append nothing (pos -1), replay nothing (valid_len 0)
-    and never flush, so the null slot is never written.
+    and never flush, so the null slot is never written;
+  * prefill() brings prompts into slots: the recurrence over all their tokens
+    (gdn_prefill), the final states quantised to the slots' checkpoints.
 """
 
 from __future__ import annotations
@@ -27,6 +29,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+import gdn_prefill as gp
 import gdn_replayssm_fp8_kernel as gk
 import gdnr_lib
 
@@ -78,6 +81,64 @@ class ReplaySSMCache:
         """End the sequence in ``slot``: its ring restarts; the slot is free."""
         self._check_slot(slot)
         self.fill[slot] = 0
+
+    def _states(self, slots: np.ndarray) -> torch.Tensor:
+        """float32 states [n, HV, V, K] of the sequences in ``slots``: their
+        checkpoints, and the ring's tokens since, one full-state step each."""
+        at = torch.from_numpy(slots).to(self.device)
+        codes = self.payload.view(torch.uint8)[at].view(FP8_DTYPE)
+        state = gk.dequantize_checkpoint(gk.QuantizedCheckpoint(codes, self.scale[at], "vblock", gk.VBLOCK, 0.0))
+        fill = self.fill[slots]
+        for t in range(int(fill.max(initial=0))):
+            # (no decay and no update where the ring is shorter, whatever it held before)
+            on = torch.from_numpy(fill > t).to(self.device)
+            k, v, g, beta = (torch.where(on.view(-1, *[1] * (ring.dim() - 2)), ring[at, t], 0.0)
+                             for ring in (self.k_ring, self.v_ring, self.g_ring, self.beta_ring))
+            gk.gdn_bf16_step(state, k, k, v, g, beta)
+        return state
+
+    def prefill(self, slots, lengths, mixed_qkv: torch.Tensor, a: torch.Tensor, b: torch.Tensor, a_log: torch.Tensor,
+                dt_bias: torch.Tensor, continued=None, out: torch.Tensor | None = None,
+                state_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Run lengths[i] packed tokens of the sequence in each slot slots[i]
+        (host ints, distinct, none the null slot): mixed_qkv [T, 2HK + HV V], a
+        and b [T, HV] of all of them, T = sum(lengths). A sequence starts from
+        nothing, or goes on from its slot where continued[i] is true (a
+        prompt's next chunk, a new turn). Afterwards the slot's checkpoint holds
+        its state and its ring is empty. Returns out [T, HV, V].
+
+        state_dtype is what the states are held in up to their quantisation.
+        float32 keeps the checkpoint the exact state's; torch.bfloat16 halves
+        the products' work with bfloat16 rows, and its rounding, an eighth of
+        e4m3's smallest, moves a code here and there by one."""
+        slots = np.asarray(slots, dtype=np.int64)
+        lengths = np.asarray(lengths, dtype=np.int64)
+        if slots.ndim != 1 or slots.shape != lengths.shape:
+            raise ValueError("slots and lengths must be one-dimensional and of one length")
+        for slot in slots:
+            self._check_slot(int(slot))
+        if np.unique(slots).size != slots.size:
+            raise ValueError("a slot appears twice in the batch")
+        if (lengths < 0).any() or int(lengths.sum()) != mixed_qkv.shape[0]:
+            raise ValueError(f"lengths must not be negative and must sum to mixed_qkv's {mixed_qkv.shape[0]} rows")
+        n = slots.size
+        goes_on = np.zeros(n, dtype=bool) if continued is None else np.asarray(continued, dtype=bool)
+        if goes_on.shape != slots.shape:
+            raise ValueError("continued must have one entry a slot")
+        # (slot 0 of the scratch is its null slot)
+        state = torch.empty(n + 1, self.value_heads, self.value_dim, self.key_dim, dtype=state_dtype, device=self.device)
+        if goes_on.any():
+            state[torch.from_numpy(np.flatnonzero(goes_on) + 1).to(self.device)] = self._states(slots[goes_on]).to(state_dtype)
+        meta = torch.from_numpy(np.concatenate([np.arange(1, n + 1), [0], np.cumsum(lengths)]).astype(np.int32)).to(self.device)
+        result = gp.gdn_prefill(mixed_qkv, a, b, a_log, dt_bias, state, meta[:n], meta[n:],
+                                has_initial_state=torch.from_numpy(goes_on).to(self.device), out=out)
+        if n:
+            ck = gk.quantize_checkpoint(state[1:], saturation=False)
+            at = torch.from_numpy(slots).to(self.device)
+            self.payload.view(torch.uint8)[at] = ck.payload.view(torch.uint8)
+            self.scale[at] = ck.scale
+            self.fill[slots] = 0
+        return result
 
     def metadata(self, slots) -> tuple[np.ndarray, np.ndarray, np.ndarray, np.ndarray]:
         """(slots, pos, valid_len, flush) of one step for the batch ``slots``
