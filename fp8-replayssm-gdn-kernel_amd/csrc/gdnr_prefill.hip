@@ -555,6 +555,31 @@ __device__ __forceinline__ float column_max(float x) {
   return __builtin_elementwise_maximum(__uint_as_float(row[0]), __uint_as_float(row[1]));
 }
 
+// Of a 16-row tile as a product leaves it (rows 4 grp + j, column lane & 15),
+// each lane's 4 rows against the columns of its 4 neighbours: row 4 grp + (lane & 3)
+// at columns lane & 12 to (lane & 12) + 3, to p (this lane's own place there),
+// rounded to the activations' type, where `in`. One store in place of four.
+template <class Act>
+__device__ __forceinline__ void store_turned(uint8_t* p, const f32x4_t& x, int lane, bool in) {
+  const bool odd = lane & 1, upper = lane & 2;
+  if constexpr (Act::kBytes == 2) {
+    auto pack = [](float lo, float hi) {
+      if constexpr (std::is_same<Act, ActBF16>::value) return pack_bf16x2(lo, hi);
+      else return pack_f16(lo, hi);
+    };
+    const uint32_t a = pack(x[0], x[1]), b = pack(x[2], x[3]);
+    const uint32_t take = odd ? 0x03020706u : 0x05040100u;  // bytes 0-3 own, 4-7 the neighbour's
+    const uint32_t r01 = __builtin_amdgcn_perm(dpp_u<kDppXor1>(a), a, take), r23 = __builtin_amdgcn_perm(dpp_u<kDppXor1>(b), b, take);
+    const uint32_t y = dpp_u<kDppXor2>(upper ? r01 : r23);
+    if (in) *(uint2*)p = upper ? make_uint2(y, r23) : make_uint2(r01, y);
+  } else {
+    const float a = dpp_f<kDppXor1>(odd ? x[0] : x[1]), b = dpp_f<kDppXor1>(odd ? x[2] : x[3]);
+    const float2 r01 = odd ? make_float2(a, x[1]) : make_float2(x[0], a), r23 = odd ? make_float2(b, x[3]) : make_float2(x[2], b);
+    const float y0 = dpp_f<kDppXor2>(upper ? r01.x : r23.x), y1 = dpp_f<kDppXor2>(upper ? r01.y : r23.y);
+    if (in) *(f32x4_t*)p = upper ? f32x4_t{y0, y1, r23.x, r23.y} : f32x4_t{r01.x, r01.y, y0, y1};
+  }
+}
+
 // KIB KiB (an even number) from memory to LDS, by COUNT waves of which this is wave w
 template <int KIB, int COUNT>
 __device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, int w) {
@@ -567,16 +592,19 @@ __device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, 
 }
 
 // LDS of the scan: a chunk's keys, scalars and T tiles twice (the next chunk's
-// arrive while this one's are used), its queries and A tiles twice, or once
-// under SPLIT, whose operands are twice as large; with ROLES the scalars again
-// beside the queries, and twice what the state's wave hands over.
-template <bool SPLIT, bool ROLES>
+// arrive while this one's are used); its queries and A tiles twice, or once
+// under SPLIT, whose operands are twice as large. With ROLES also the chunk's v
+// twice, and what the state's wave hands over (4 operands of S, 2 of U, scale
+// and first bad token; SPLIT: once).
+template <bool SPLIT, bool ROLES, int ES>
 struct ScanLds {
   static constexpr int KEYS = (int)(plane_bytes(SPLIT) + kScalars + tri_bytes(SPLIT));
-  static constexpr int QUERIES = (int)(plane_bytes(SPLIT) + tri_bytes(SPLIT)) + (ROLES ? kScalars : 0);
-  static constexpr int QBUFS = SPLIT ? 1 : 2;
-  static constexpr int HANDED = ROLES ? 7 * 1024 : 0;  // 4 operands of S, 2 of U, scale and first bad token
-  static constexpr int BYTES = 2 * KEYS + QBUFS * QUERIES + 2 * HANDED;
+  static constexpr int QUERIES = (int)(plane_bytes(SPLIT) + tri_bytes(SPLIT));
+  static constexpr int VALUES = ROLES ? C * 16 * ES : 0;
+  static constexpr int HANDED = ROLES ? (SPLIT ? 13 : 7) * 1024 : 0;
+  static constexpr int BUFS = SPLIT ? 1 : 2;  // of queries and of what is handed over
+  static constexpr int QUERIES_AT = 2 * KEYS, VALUES_AT = QUERIES_AT + BUFS * QUERIES, HANDED_AT = VALUES_AT + 2 * VALUES;
+  static constexpr int BYTES = HANDED_AT + BUFS * HANDED;
 };
 
 // A sequence's chunks in order. A wave has 16 V-rows of one value head, the
@@ -586,20 +614,22 @@ struct ScanLds {
 // the keys', queries', T's and A's fragments are read in that one.
 //
 // The chain over the chunks is the state's: K S0^T, R, U, S1. The outputs hang
-// off it. With ROLES (two waves a workgroup) one wave carries the chain and
+// off it. With ROLES (three waves a workgroup) one wave carries the chain and
 // hands S0's and U's operands through LDS to a second one, which forms the
-// outputs of chunk c while the first is at chunk c + 1; otherwise WAVES waves
-// do both for 16 V-rows each on shared operands.
+// outputs of chunk c while the first is at chunk c + 1; a third fetches what
+// either reads (48 copies a chunk, whose issue alone costs a wave 850 cycles).
+// Otherwise WAVES waves do all of it for 16 V-rows each on shared operands.
 template <class Act, class St, bool SPLIT, int WAVES, bool ROLES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_scan_kernel(const PrefillArgs a) {
-  using L = ScanLds<SPLIT, ROLES>;
-  constexpr int ES = Act::kBytes, P = SPLIT ? 2 : 1, RS = 2 * K, COLS = ROLES ? 16 : 16 * WAVES;
+  constexpr int ES = Act::kBytes;
+  using L = ScanLds<SPLIT, ROLES, ES>;
+  constexpr int RS = 2 * K, COLS = ROLES ? 16 : 16 * WAVES;
   constexpr float kUp = SPLIT ? kFix : 1.f, kDown = 1.f / kUp;
-  static_assert(!ROLES || (WAVES == 2 && !SPLIT), "one wave a role");
+  static_assert(!ROLES || WAVES == 3, "one wave a role");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const bool chain = !ROLES || wave == 0, outputs = !ROLES || wave == 1;
+  const bool chain = !ROLES || wave == 0, outputs = !ROLES || wave == 1, fetches = !ROLES || wave == 2;
   // Workgroups go to the 8 XCDs in turn: those of one key head, which read the
   // same keys and queries, to one of them.
   const int blocks = a.V / COLS, n = blockIdx.y;
@@ -633,12 +663,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     dma_part<(int)plane_bytes(SPLIT) / 1024, kTeam>(unit + c * unit_step, to, member);
     dma_part<(int)(kScalars + tri_bytes(SPLIT)) / 1024, kTeam>(head + c * head_step, to + plane_bytes(SPLIT), member);
   };
-  auto queries_at = [&](int c) { return 2 * L::KEYS + (L::QBUFS == 2 ? (c & 1) * L::QUERIES : 0); };
+  auto queries_at = [&](int c) { return L::QUERIES_AT + (c % L::BUFS) * L::QUERIES; };
   auto fetch_queries = [&](int c) {
     const uint32_t to = lds0 + queries_at(c);
     dma_part<(int)plane_bytes(SPLIT) / 1024, kTeam>(unit + c * unit_step + plane_bytes(SPLIT), to, member);
     dma_part<(int)tri_bytes(SPLIT) / 1024, kTeam>(head + c * head_step + kScalars + tri_bytes(SPLIT), to + plane_bytes(SPLIT), member);
-    if constexpr (ROLES) dma_part<kScalars / 1024, kTeam>(head + c * head_step, to + plane_bytes(SPLIT) + tri_bytes(SPLIT), member);
   };
   // 16 tokens by 32 columns k of keys or queries at b
   auto rows_of = [&](const uint8_t* b, int tile, int step) {
@@ -694,10 +723,17 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   const int64_t v_row = a.mx_t * ES, o_row = a.o_t * ES;
   const uint8_t* vp = (const uint8_t*)a.mixed + (int64_t)begin * v_row + (2 * a.H * K + hv * a.V) * ES;
   uint8_t* op = (uint8_t*)a.out + (int64_t)begin * o_row + hv * a.o_h * ES;
-  const uint32_t v_lane = (uint32_t)(4 * grp * v_row) + v0 * ES, o_lane = (uint32_t)(4 * grp * o_row) + v0 * ES;
+  const uint32_t v_lane = (uint32_t)(4 * grp * v_row) + v0 * ES, o_lane = (uint32_t)((4 * grp + (lane & 3)) * o_row) + (v0 & ~3) * ES;
   auto fetch_v = [&](int c) {
     const uint8_t* p = vp + c * C * v_row;
-    if ((c + 1) * C <= len) {
+    if constexpr (ROLES) {  // rows of 16 V-rows' values, to LDS
+#pragma unroll
+      for (int i = 0; i < ES; ++i) {
+        const int x = 64 * i + lane, t = x / ES;
+        dma16(p + (uint32_t)min(t, len - 1 - c * C) * v_row + (v0 - col) * ES + 16 * (x % ES),
+              lds0 + L::VALUES_AT + (c & 1) * L::VALUES + 1024 * i);
+      }
+    } else if ((c + 1) * C <= len) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) vn[i] = Act::ld_bits(p + (16 * (i >> 2) + (i & 3)) * v_row + v_lane, 0);
     } else {
@@ -707,6 +743,15 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   };
   bool any_bad = false;
   int first = C;  // first token of the chunk whose results are NaN in this V-row
+
+  // what is handed over: operands of S (0 .. 3) and U (4, 5), then scale and first
+  // bad token; SPLIT: the operands' low halves after that
+  auto place = [&](int c, int i) { return (u32x4_t*)(lds + L::HANDED_AT + (c % L::BUFS) * L::HANDED + 1024 * i + 16 * lane); };
+  constexpr int kLow = 7;
+  auto hand_over = [&](int c, int i, const Operand<SPLIT>& o) {
+    *place(c, i) = o.hi;
+    if constexpr (SPLIT) *place(c, kLow + i) = o.lo;
+  };
 
   // the chain: chunk c's R and U from S, then S after it
   auto state_step = [&](int c) {
@@ -732,20 +777,31 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const float total = scal[4 * C - 1];
     const int bad_token = __builtin_amdgcn_readfirstlane(((const int*)scal)[4 * C]);
     float v[4][4];
+    if constexpr (ROLES) {
+      const uint8_t* p = lds + L::VALUES_AT + (c & 1) * L::VALUES;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = Act::from_bits(vn[i]);
+      for (int tt = 0; tt < 4; ++tt) {
+        if constexpr (ES == 2) {
+          const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 32 * (16 * tt + 4 * grp + (col >> 2)) + 8 * (col & 3))));
+          const float2 lo = Act::from_pair(x.x), hi = Act::from_pair(x.y);
+          v[tt][0] = lo.x, v[tt][1] = lo.y, v[tt][2] = hi.x, v[tt][3] = hi.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[tt][j] = *(const float*)(p + 64 * (16 * tt + 4 * grp + j) + 4 * col);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = Act::from_bits(vn[i]);
+    }
     if ((c + 1) * C > len) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (c * C + 16 * (i >> 2) + 4 * grp + (i & 3) >= len) v[i >> 2][i & 3] = 0.f;
     }
-    if (c + 1 < chunks) {
-      fetch_v(c + 1);
-      GDNR_COMPILER_FENCE();
-      if constexpr (SPLIT) fetch_queries(c);
-      fetch_keys(c + 1);
-    } else if constexpr (SPLIT) {
-      fetch_queries(c);
+    if constexpr (!ROLES) {
+      if (SPLIT) fetch_queries(c);
+      if (c + 1 < chunks) fetch_keys(c + 1), fetch_v(c + 1);
     }
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) read_rows(b, s);
@@ -795,7 +851,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       for (int kt = 0; kt < 8; ++kt) S[kt] *= ratio;
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s) bs[s] = operand<SPLIT>(S[2 * s], S[2 * s + 1]);
+    for (int s = 0; s < 4; ++s) {
+      bs[s] = operand<SPLIT>(S[2 * s], S[2 * s + 1]);
+      if constexpr (ROLES) hand_over(c, s, bs[s]);
+    }
+    if constexpr (ROLES) *place(c, 6) = u32x4_t{__float_as_uint(inv), (uint32_t)first, any_bad, 0};
 
     f32x4_t u[4];
     by_state(b, u);  // K S0^T
@@ -837,6 +897,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     for (int s = 0; s < 2; ++s) {
       ud[s] = operand<SPLIT>(u[2 * s] * ed[2 * s], u[2 * s + 1] * ed[2 * s + 1]);
       ub[s] = operand<SPLIT>(u[2 * s], u[2 * s + 1]);
+      if constexpr (ROLES) hand_over(c, 4 + s, ub[s]);
     }
     // the state after the chunk, KT tiles of one half of the tokens at a time
 #pragma unroll
@@ -862,16 +923,19 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     }
   };
 
-  // the outputs of chunk c from bs, ub, inv, first and any_bad
-  auto output_step = [&](int c) {
-    const uint8_t* b = lds + queries_at(c);
-    const float* scal = (const float*)(ROLES ? b + plane_bytes(SPLIT) + tri_bytes(SPLIT) : lds + (c & 1) * L::KEYS + plane_bytes(SPLIT));
-    const f32x4_t* grow4 = (const f32x4_t*)(scal + 3 * C);
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) read_rows(b, s);
-    f32x4_t o[4], gr[4];
+  // the outputs of chunk c from bs, ub, inv, first, any_bad and e^G (gr)
+  f32x4_t gr[4];
+  auto read_grow = [&](int c) {
+    const f32x4_t* grow4 = (const f32x4_t*)(lds + (c & 1) * L::KEYS + plane_bytes(SPLIT) + 3 * C * 4);
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) gr[tt] = grow4[4 * tt + grp];
+  };
+  auto output_step = [&](int c) {
+    const uint8_t* b = lds + queries_at(c);
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) read_rows(b, s);
+    f32x4_t o[4];
+    if constexpr (!ROLES) read_grow(c);
     GDNR_COMPILER_FENCE();
     if constexpr (!SPLIT) read_triangle(b + plane_bytes(SPLIT));
     by_state(b, o);  // Q S0^T
@@ -889,17 +953,17 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     }
     // (what is on its way to LDS is waited for before the stores, which then
     // have a whole chunk to drain)
-    GDNR_WAIT_VMCNT(0);
-    uint8_t* orow = op + c * C * o_row;
-    auto store = [&](int i) { Act::st(orow + (16 * (i >> 2) + (i & 3)) * o_row + o_lane, 0, o[i >> 2][i & 3]); };
-    if ((c + 1) * C <= len) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) store(i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c * C + 16 * (i >> 2) + (i & 3) + 4 * grp < len) store(i);
+    if constexpr (!ROLES) {
+      GDNR_WAIT_VMCNT(0);
+    } else if (L::BUFS == 1 && c + 1 < chunks) {
+      GDNR_WAIT_LGKM0();  // (this chunk's have been read)
+      fetch_queries(c + 1);
+      GDNR_WAIT_VMCNT(0);
     }
+    uint8_t* orow = op + c * C * o_row + o_lane;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+      store_turned<Act>(orow + 16 * tt * o_row, o[tt], lane, c * C + 16 * tt + 4 * grp + (lane & 3) < len);
   };
 
   if (chain) {
@@ -910,36 +974,45 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
       for (int j = 0; j < 4; ++j) S[kt][j] = started ? x[j] : 0.f;
     }
-    if (chunks) fetch_keys(0), fetch_v(0);
-    if (!ROLES && !SPLIT && chunks) fetch_queries(0);
-    GDNR_WAIT_VMCNT(0);
   }
+  if (fetches && chunks) {
+    fetch_keys(0), fetch_v(0);
+    if (!ROLES && !SPLIT) fetch_queries(0);
+  }
+  GDNR_WAIT_VMCNT(0);
   if constexpr (ROLES) {
     for (int c = 0; c <= chunks; ++c) {
-      __syncthreads();  // chunk c - 1 is handed over; what it read may be overwritten
-      uint8_t* handed = lds + 2 * L::KEYS + L::QBUFS * L::QUERIES + 16 * lane;
+      __syncthreads();  // chunk c's keys and v are in LDS, chunk c - 1 is handed over
+      if (outputs) {
+        if (c > 0) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            bs[s].hi = *place(c - 1, s);
+            if constexpr (SPLIT) bs[s].lo = *place(c - 1, kLow + s);
+          }
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            ub[s].hi = *place(c - 1, 4 + s);
+            if constexpr (SPLIT) ub[s].lo = *place(c - 1, kLow + 4 + s);
+          }
+          const u32x4_t x = *place(c - 1, 6);
+          inv = __uint_as_float(x[0]), first = (int)x[1], any_bad = __builtin_amdgcn_readfirstlane(x[2]) != 0;
+        }
+        if (L::BUFS == 1 && c == 0 && chunks) fetch_queries(0);
+      }
+      if constexpr (L::BUFS == 1) __syncthreads();  // what was handed over is in registers
       if (chain && c < chunks) {
         state_step(c);
-        u32x4_t* to = (u32x4_t*)(handed + (c & 1) * L::HANDED);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) to[64 * s] = bs[s].hi;
-        to[64 * 4] = ub[0].hi, to[64 * 5] = ub[1].hi;
-        to[64 * 6] = u32x4_t{__float_as_uint(inv), (uint32_t)first, any_bad, 0};
-        GDNR_WAIT_VMCNT(0);
       }
       if (outputs) {
-        if (c < chunks) fetch_queries(c);
-        if (c > 0) {
-          const u32x4_t* from = (const u32x4_t*)(handed + ((c - 1) & 1) * L::HANDED);
-#pragma unroll
-          for (int s = 0; s < 4; ++s) bs[s].hi = from[64 * s];
-          ub[0].hi = from[64 * 4], ub[1].hi = from[64 * 5];
-          const u32x4_t x = from[64 * 6];
-          inv = __uint_as_float(x[0]), first = (int)x[1], any_bad = __builtin_amdgcn_readfirstlane(x[2]) != 0;
-          output_step(c - 1);
-        } else {
-          GDNR_WAIT_VMCNT(0);
-        }
+        if (c > 0) output_step(c - 1);
+        else GDNR_WAIT_VMCNT(0);
+        if (c < chunks) read_grow(c);
+      }
+      if (fetches) {
+        if (c + 1 < chunks) fetch_keys(c + 1), fetch_v(c + 1);
+        if (L::BUFS == 2 && c < chunks) fetch_queries(c);
+        GDNR_WAIT_VMCNT(0);
       }
     }
   } else {
@@ -981,7 +1054,7 @@ int launch_prep(const PrefillArgs& a, hipStream_t s) {
 }
 template <class Act, class St, bool SPLIT, int WAVES, bool ROLES>
 int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
-  constexpr int lds = ScanLds<SPLIT, ROLES>::BYTES;
+  constexpr int lds = ScanLds<SPLIT, ROLES, Act::kBytes>::BYTES;
   static_assert(lds <= kMaxStepLds, "the operands fit");
   const auto kernel = chunk_scan_kernel<Act, St, SPLIT, WAVES, ROLES>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -991,22 +1064,28 @@ int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
 }
 // A workgroup's LDS leaves room for one on a compute unit, so the scan's time is
 // the rounds its workgroups take over the card times what a chunk costs them:
-// with 8 waves (128 V-rows) 3.7 us, 4 waves 2.8, one and its outputs' wave
-// (16 V-rows) 2.0; with SPLIT operands 7.0 and 5.0, and with 2 waves (32
-// V-rows) 4.7. The cheapest product runs, the wider one of equals (it reads the
-// operands once for more rows). us a call of 1024 tokens a sequence, HV=32,
-// V=128, with 8 waves, 4 and the pair: 2 sequences 81, 65 and 77; 4: 91, 79 and
-// 136; 6: 113, 133 and 202; 8: 128, 144 and 266.
+// with 8 waves (128 V-rows) 3.7 us, 4 waves 2.8, the three roles (16 V-rows) 1.4;
+// with SPLIT operands 7.0, 5.0 and 3.3, and with 2 waves (32 V-rows) 4.7. The
+// cheapest product runs, the wider one of equals (it reads the operands once for
+// more rows). us a call of 1024 tokens a sequence, HV=32, V=128, with 8 waves, 4
+// and the roles: 1 sequence 78, 62 and 47; 2: 80, 65 and 73; 4: 88, 75 and 124;
+// 6: 109, 133 and 186; 8: 127, 147 and 238. f16 with an f32 state, HV=12, 512
+// tokens a sequence, with 4 waves, 2 and the roles: 1 sequence 63, 59 and 46; 4:
+// 67, 65 and 71; 16: 137, 164 and 185, with 8 waves 105.
 template <class Act, class St, bool SPLIT>
 int launch_scan(const PrefillArgs& a, hipStream_t s) {
   const int64_t rows = (int64_t)a.N * a.HV * a.V, cus = device_cus();
   const auto cost = [&](int columns, int chunk) {
     return a.V % columns ? INT64_MAX : (rows / columns + cus - 1) / cus * chunk;
   };
-  const int64_t eight = cost(128, SPLIT ? 70 : 37), four = cost(64, SPLIT ? 50 : 28), thin = cost(SPLIT ? 32 : 16, SPLIT ? 47 : 20);
-  if (eight <= four && eight <= thin) return launch_scan_as<Act, St, SPLIT, 8, false>(a, s);
-  if (four <= thin) return launch_scan_as<Act, St, SPLIT, 4, false>(a, s);
-  return launch_scan_as<Act, St, SPLIT, 2, !SPLIT>(a, s);
+  const int64_t eight = cost(128, SPLIT ? 70 : 37), four = cost(64, SPLIT ? 50 : 28), one = cost(16, SPLIT ? 33 : 14);
+  if constexpr (SPLIT) {
+    const int64_t two = cost(32, 47);
+    if (two <= one && two < four && two < eight) return launch_scan_as<Act, St, SPLIT, 2, false>(a, s);
+  }
+  if (eight <= four && eight <= one) return launch_scan_as<Act, St, SPLIT, 8, false>(a, s);
+  if (four <= one) return launch_scan_as<Act, St, SPLIT, 4, false>(a, s);
+  return launch_scan_as<Act, St, SPLIT, 3, true>(a, s);
 }
 
 template <class Act, class St, bool GATE_F32>
