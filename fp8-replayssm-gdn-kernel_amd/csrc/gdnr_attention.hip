@@ -129,6 +129,9 @@ __device__ __forceinline__ int sequences_up_to(const AttentionArgs& a, int x, in
   return count;
 }
 
+struct Block {  // a workgroup's place in its kernel's grid, or that grid
+  int x, y, z;
+};
 struct Span {
   int begin, end, context;
 };
@@ -167,25 +170,24 @@ constexpr int lds_bytes() {
 // its values once the outputs have; two to four workgroups a compute unit
 // cover the waits.
 template <class Act, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 ? 4 : 2))) void few_kernel(const AttentionArgs a) {
+__device__ __forceinline__ void few_step(const AttentionArgs& a, uint8_t* lds, const Block blk) {
   constexpr int KSTEPS = D / 32, DT = D / 16, PPR = D / 8, RPI = 64 / PPR, NV = kKeys / RPI;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int gt = min(a.G, kRows), tb = kRows / gt;  // heads and tokens of a tile
   // beside tile_kernel, one tile holds all rows of each sequence that is taken here
-  int n = blockIdx.y;
+  int n = blk.y;
   if (a.few_rows > kRows) n = sequences_up_to(a, n, tb, 1) - 1;
   if (n < 0) return;
   const Span sq = span_of(a, n);
-  const int tok0 = a.few_rows > kRows ? sq.begin + ((int)blockIdx.y - sq.begin / tb - n) * tb : sq.begin;
+  const int tok0 = a.few_rows > kRows ? sq.begin + (blk.y - sq.begin / tb - n) * tb : sq.begin;
   if (tok0 >= sq.end || !few_rows(a, sq)) return;
   const int head_tiles = (a.G + kRows - 1) / kRows;
-  const int hk = blockIdx.x / head_tiles, ht = blockIdx.x - hk * head_tiles;
+  const int hk = blk.x / head_tiles, ht = blk.x - hk * head_tiles;
   const int last = min(tok0 + tb, sq.end) - 1;
   const int piece = a.piece[0], pieces = a.pieces[0];
-  const int k_begin = (int)blockIdx.z * piece, k_end = min(visible(sq, last), k_begin + piece);
-  if (k_begin >= k_end && (pieces > 1 || blockIdx.z > 0)) return;
+  const int k_begin = blk.z * piece, k_end = min(visible(sq, last), k_begin + piece);
+  if (k_begin >= k_end && (pieces > 1 || blk.z > 0)) return;
 
   // this lane's row
   const int rt = tok0 + col / gt, rh = ht * kRows + col % gt;
@@ -369,13 +371,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 
     for (int w = 0; w < kWaves; ++w) sum += f[w] * *(const f32x4_t*)(lds + (w * kRows + row) * o_stride<D>() + 4 * d);
     sum *= norm;
     if (pieces > 1) {
-      *(f32x4_t*)(a.part + (((int64_t)blockIdx.z * a.T + t) * a.HQ + qh) * D + d) = sum;
+      *(f32x4_t*)(a.part + (((int64_t)blk.z * a.T + t) * a.HQ + qh) * D + d) = sum;
     } else {
       *(uint2*)((uint8_t*)a.out + (t * a.o_t + qh * a.o_h + d) * 2) = make_uint2(pack2<Act>(sum[0], sum[1]), pack2<Act>(sum[2], sum[3]));
     }
   }
   if (pieces > 1 && dl == 0) {
-    float* p = a.part_ml + (((int64_t)blockIdx.z * a.T + t) * a.HQ + qh) * 2;
+    float* p = a.part_ml + (((int64_t)blk.z * a.T + t) * a.HQ + qh) * 2;
     p[0] = top, p[1] = l;
   }
 }
@@ -394,26 +396,25 @@ struct Tile {
 // queries, scores and outputs in registers; the keys' fragment it reads from
 // LDS serves both of its row tiles.
 template <class Act, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(const AttentionArgs a) {
+__device__ __forceinline__ void tile_step(const AttentionArgs& a, uint8_t* lds, const Block blk) {
   using TL = Tile<D>;
   constexpr int KSTEPS = D / 32, DT = D / 16, NT = TL::NT, KEYS = TL::KEYS, MT = KEYS / 16, PPR = D / 8;
   constexpr int RPI = 64 / PPR;                     // rows of an LDS copy
   constexpr int COPIES = KEYS / RPI / kWaves;       // copies of keys (and of values) a wave and step
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int gt = min(a.G, TL::ROWS), tb = TL::ROWS / gt;  // heads and tokens of a workgroup
-  const int n = sequences_up_to(a, blockIdx.y, tb, 1) - 1;
+  const int n = sequences_up_to(a, blk.y, tb, 1) - 1;
   if (n < 0) return;
   const Span sq = span_of(a, n);
-  const int tok0 = sq.begin + ((int)blockIdx.y - sq.begin / tb - n) * tb;
+  const int tok0 = sq.begin + (blk.y - sq.begin / tb - n) * tb;
   if (tok0 >= sq.end || few_rows(a, sq)) return;
   const int head_tiles = (a.G + TL::ROWS - 1) / TL::ROWS;
-  const int hk = blockIdx.x / head_tiles, ht = blockIdx.x - hk * head_tiles;
+  const int hk = blk.x / head_tiles, ht = blk.x - hk * head_tiles;
   const int last = min(tok0 + tb, sq.end) - 1;
   const int piece = a.piece[1], pieces = a.pieces[1];
-  const int k_begin = (int)blockIdx.z * piece, k_end = min(visible(sq, last), k_begin + piece);
-  if (k_begin >= k_end && (pieces > 1 || blockIdx.z > 0)) return;
+  const int k_begin = blk.z * piece, k_end = min(visible(sq, last), k_begin + piece);
+  if (k_begin >= k_end && (pieces > 1 || blk.z > 0)) return;
 
   // this lane's rows
   int rt[NT], rh[NT], vis[NT];
@@ -665,7 +666,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (!live[nt]) continue;
     const int qh = hk * a.G + rh[nt];
     if (pieces > 1) {
-      const int64_t at = ((int64_t)blockIdx.z * a.T + rt[nt]) * a.HQ + qh;
+      const int64_t at = ((int64_t)blk.z * a.T + rt[nt]) * a.HQ + qh;
 #pragma unroll
       for (int i = 0; i < DT; ++i) *(f32x4_t*)(a.part + at * D + 16 * i + 4 * grp) = o[nt][i];
       if (grp == 0) a.part_ml[2 * at] = m_run[nt], a.part_ml[2 * at + 1] = l;
@@ -679,6 +680,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
   }
+}
+
+// The kernels: each walk alone, or both in one launch (the tiles' workgroups
+// first) where a batch has sequences of either kind: the few rows' latency then
+// hides behind the tiles' products (16 sequences, three of them with 400 tokens,
+// 50.5 us a call in two launches, 39.7 in one).
+template <class Act, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, D == 64 ? 4 : 2))) void few_kernel(const AttentionArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  few_step<Act, D>(a, lds, Block{(int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z});
+}
+template <class Act, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(const AttentionArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  tile_step<Act, D>(a, lds, Block{(int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z});
+}
+// few and tile: the two grids, x fastest
+template <class Act, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void both_kernel(const AttentionArgs a, const Block few, const Block tile) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const auto block = [](int i, const Block& grid) {
+    const int row = i / grid.x, z = row / grid.y;
+    return Block{i - row * grid.x, row - z * grid.y, z};
+  };
+  const int tiles = tile.x * tile.y * tile.z, i = blockIdx.x;
+  if (i < tiles) tile_step<Act, D>(a, lds, block(i, tile));
+  else few_step<Act, D>(a, lds, block(i - tiles, few));
 }
 
 // The pieces of a row joined in their order. D / 4 lanes a row, the rows of a
@@ -740,24 +768,27 @@ int launch_dim(const AttentionArgs& a, hipStream_t s) {
   const auto grid = [&](int rows, int pieces) {  // key heads first: a head's workgroups share an XCD
     const int gt = a.G < rows ? a.G : rows, tb = rows / gt;
     const bool one_tile = rows == kRows && a.few_rows == kRows;
-    return dim3(a.HKV * ((a.G + rows - 1) / rows), one_tile ? a.N : a.T / tb + a.N, pieces);
+    return Block{a.HKV * ((a.G + rows - 1) / rows), one_tile ? a.N : a.T / tb + a.N, pieces};
   };
-  const auto launch = [&](auto kernel, int rows, int pieces, int lds) {
+  const auto launch = [&](auto kernel, dim3 blocks, int lds, auto... more) {
     if (lds > 64 * 1024) {  // (enabled per kernel and device; idempotent, cheap)
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(kernel, grid(rows, pieces), dim3(256), lds, s, a);
+    hipLaunchKernelGGL(kernel, blocks, dim3(256), lds, s, a, more...);
     return (int)hipGetLastError();
   };
-  if (a.pieces[0]) {
-    const int rc = launch(few_kernel<Act, D>, kRows, a.pieces[0], lds_bytes<D>());
-    if (rc) return rc;
+  constexpr int few_lds = lds_bytes<D>(), tile_lds = Tile<D>::LDS;
+  const Block few = grid(kRows, a.pieces[0]), tile = grid(Tile<D>::ROWS, a.pieces[1]);
+  const int64_t fews = (int64_t)few.x * few.y * few.z, tiles = (int64_t)tile.x * tile.y * tile.z;
+  int rc = 0;
+  if (fews && tiles && fews + tiles < 1 << 24) {  // (a dimension of a grid ends at 2^32 threads)
+    rc = launch(both_kernel<Act, D>, dim3((uint32_t)(fews + tiles)), few_lds > tile_lds ? few_lds : tile_lds, few, tile);
+  } else {
+    if (fews) rc = launch(few_kernel<Act, D>, dim3(few.x, few.y, few.z), few_lds);
+    if (!rc && tiles) rc = launch(tile_kernel<Act, D>, dim3(tile.x, tile.y, tile.z), tile_lds);
   }
-  if (a.pieces[1]) {
-    const int rc = launch(tile_kernel<Act, D>, Tile<D>::ROWS, a.pieces[1], Tile<D>::LDS);
-    if (rc) return rc;
-  }
+  if (rc) return rc;
   if (a.pieces[0] > 1 || a.pieces[1] > 1) {
     constexpr int R = 256 / D;  // heads a wave
     hipLaunchKernelGGL((join_kernel<Act, D>), dim3(a.T, (a.HQ + 4 * R - 1) / (4 * R)), dim3(256), 0, s, a);
