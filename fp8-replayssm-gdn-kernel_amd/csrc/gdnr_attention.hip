@@ -810,7 +810,11 @@ int launch_act(const AttentionArgs& a, hipStream_t s) {
 // them; a single longer one is tile_kernel's; otherwise each takes its kind. A
 // context is cut while a kernel would have fewer than eight (few) or two
 // (tile) workgroups a compute unit, into whole steps of 128 keys, at least 256:
-// a shorter piece costs as much to join as to walk.
+// a shorter piece costs as much to join as to walk. us a call with half, this and
+// twice as many workgroups: 64 decodes 145, 144 and 150; three chunks of 400
+// tokens beside 13 decodes 46.5, 39.8 and 40.2; a chunk of 2048 tokens 269 as it
+// is (one piece) and 302 with twice as many. One decode over 8192 keys with
+// pieces of 256 keys 12.6, of 128 14.2.
 void plan_attention(AttentionArgs* a) {
   const int64_t cus = device_cus(), rows = (int64_t)a->T * (a->G < kRows ? a->G : kRows);
   const bool all_few = rows <= (int64_t)kRows * a->N, all_tile = !all_few && a->N == 1;

@@ -591,6 +591,22 @@ __device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, 
   }
 }
 
+// The sequence at a place of the launch's order: of each 64, the longest first.
+// Workgroups start in order as others end, so that the last to start are then
+// short ones (24 sequences of up to 1096 tokens: the scan 186 us as given, 168 so).
+__device__ __forceinline__ int longest_first(const PrefillArgs& a, int place) {
+  const int lane = threadIdx.x & 63, base = place & ~63, count = min(64, a.N - base);
+  uint32_t key = 0;  // by length, then by index
+  if (lane < count) {
+    const int64_t at = (base + lane) * a.cu_s;
+    const int begin = min(max(a.cu[at], 0), a.T), end = min(max(a.cu[at + a.cu_s], begin), a.T);
+    key = (uint32_t)(end - begin) * 64 + 64 - lane;
+  }
+  int longer = 0;
+  for (int j = 0; j < count; ++j) longer += __builtin_amdgcn_readlane(key, j) > key;
+  return __builtin_amdgcn_readfirstlane(base + __builtin_ctzll(__ballot(lane < count && longer == place - base)));
+}
+
 // LDS of the scan: a chunk's keys, scalars and T tiles twice (the next chunk's
 // arrive while this one's are used); its queries and A tiles twice, or once
 // under SPLIT, whose operands are twice as large. With ROLES also the chunk's v
@@ -632,7 +648,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   const bool chain = !ROLES || wave == 0, outputs = !ROLES || wave == 1, fetches = !ROLES || wave == 2;
   // Workgroups go to the 8 XCDs in turn: those of one key head, which read the
   // same keys and queries, to one of them.
-  const int blocks = a.V / COLS, n = blockIdx.y;
+  const int blocks = a.V / COLS, n = longest_first(a, blockIdx.y);
   int unit_id = blockIdx.x;
   if (a.H % 8 == 0) {
     const int per = a.G * blocks, j = unit_id >> 3;
