@@ -287,3 +287,34 @@ def test_repeatable(device):
     want, state = run(x), x["state"].clone()
     x["state"].copy_(first)
     assert torch.equal(run(x), want) and torch.equal(x["state"], state)
+
+
+def sizes(count, low, high, seed):
+    return np.random.RandomState(seed).randint(low, high, count).tolist()
+
+
+@pytest.mark.parametrize("count,value_heads,act,state", [
+    (2, 16, BF16, BF16), (7, 8, BF16, BF16), (20, 8, BF16, BF16), (70, 4, BF16, BF16),  # 3 roles, 4 waves, 8 waves
+    (2, 16, F16, F32), (6, 8, F16, F32), (12, 8, F32, F32), (70, 4, F16, F16)])         # 3 roles, 2 waves, 4, 8
+def test_scan_forms(device, count, value_heads, act, state):
+    """Every width of the scan, each with empty sequences, single tokens and
+    lengths that tie; 70 sequences are two groups of its longest-first order."""
+    lengths = sizes(count, 20, 150, count)
+    lengths[0], lengths[count // 2], lengths[-1] = 64, 0 if count > 2 else 1, 64
+    check(make(lengths, device, seed=count, heads=value_heads // 2, value_heads=value_heads, act=act, state=state))
+
+
+def test_order_of_the_batch(device):
+    """What a sequence gets does not depend on where it stands in the batch."""
+    lengths = [70, 200, 1, 130, 64]
+    x = make(lengths, device, seed=40)
+    whole = run(x)
+    rows = torch.split(torch.arange(sum(lengths), device=device), lengths)
+    order = [3, 0, 4, 2, 1]
+    y = make(lengths, device, seed=40)
+    at = torch.cat([rows[i] for i in order])
+    for name in ("mixed", "a", "b"):
+        y[name] = y[name][at]
+    y["slots"] = y["slots"][order]
+    y["cu"] = torch.tensor(np.concatenate([[0], np.cumsum([lengths[i] for i in order])]), dtype=torch.int32, device=device)
+    assert torch.equal(run(y), whole[at]) and torch.equal(y["state"], x["state"])
