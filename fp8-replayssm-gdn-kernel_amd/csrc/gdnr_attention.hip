@@ -20,7 +20,7 @@
 // over 8192 keys 8.5 us, the chain lengths -> pages -> keys -> values.
 // tile_kernel: the others. Bound by the matrix products and the exponentials:
 // 128 rows a workgroup (64 at D = 256), 32 (16) a wave, all on the same keys.
-// 2048 tokens over 8192 keys, 32 heads of 128: 264 us, 911 TFLOP/s (a square
+// 2048 tokens over 8192 keys, 32 heads of 128: 248 us, 969 TFLOP/s (a square
 // product of 8192 in the library: 1130).
 // A context is cut into pieces where the rows alone do not fill the card, and
 // join_kernel adds the pieces in their order.
@@ -411,8 +411,16 @@ __device__ __forceinline__ void tile_step(const AttentionArgs& a, uint8_t* lds, 
   const int n = sequences_up_to(a, blk.y, tb, 1) - 1;
   if (n < 0) return;
   const Span sq = span_of(a, n);
-  const int tok0 = sq.begin + (blk.y - sq.begin / tb - n) * tb;
-  if (tok0 >= sq.end || few_rows(a, sq)) return;
+  // Later tokens see more keys: the last tile first, so that the last to start
+  // are short; and where two workgroups share a compute unit, the second ones in
+  // the other direction, the longest beside the shortest. us a call, first tile
+  // first, last first, and so, 32 heads of 128: 4096 tokens 196, 169 and 164; 2048
+  // over 8192 keys 266, 257 and 248.
+  const int tiles = (sq.end - sq.begin + tb - 1) / tb;
+  int place = blk.y - sq.begin / tb - n;
+  if (place >= tiles || few_rows(a, sq)) return;
+  if (place >= a.turn && place < 2 * a.turn) place = a.turn + min(2 * a.turn, tiles) - 1 - place;
+  const int tok0 = sq.begin + (tiles - 1 - place) * tb;
   const int head_tiles = (a.G + TL::ROWS - 1) / TL::ROWS;
   const int hk = blk.x / head_tiles, ht = blk.x - hk * head_tiles;
   const int last = min(tok0 + tb, sq.end) - 1;
@@ -768,7 +776,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttentionArgs a) {
 }
 
 template <class Act, int D>
-int launch_dim(const AttentionArgs& a, hipStream_t s) {
+int launch_dim(AttentionArgs a, hipStream_t s) {
   const auto grid = [&](int rows, int pieces) {  // key heads first: a head's workgroups share an XCD
     const int gt = a.G < rows ? a.G : rows, tb = rows / gt;
     const bool one_tile = rows == kRows && a.few_rows == kRows;
@@ -784,6 +792,8 @@ int launch_dim(const AttentionArgs& a, hipStream_t s) {
   };
   constexpr int few_lds = lds_bytes<D>(), tile_lds = Tile<D>::LDS;
   const Block few = grid(kRows, a.pieces[0]), tile = grid(Tile<D>::ROWS, a.pieces[1]);
+  if (a.N == 1 && a.pieces[1] == 1)  // (the second of two to a compute unit start there)
+    a.turn = device_cus() / tile.x;
   const int64_t fews = (int64_t)few.x * few.y * few.z, tiles = (int64_t)tile.x * tile.y * tile.z;
   int rc = 0;
   if (fews && tiles && fews + tiles < 1 << 24) {  // (a dimension of a grid ends at 2^32 threads)
@@ -816,9 +826,9 @@ int launch_act(const AttentionArgs& a, hipStream_t s) {
 // (tile) workgroups a compute unit, into whole steps of 128 keys, at least 256:
 // a shorter piece costs as much to join as to walk. us a call with half, this and
 // twice as many workgroups: 64 decodes 145, 144 and 150; three chunks of 400
-// tokens beside 13 decodes 46.5, 39.8 and 40.2; a chunk of 2048 tokens 269 as it
-// is (one piece) and 302 with twice as many. One decode over 8192 keys with
-// pieces of 256 keys 12.6, of 128 14.2.
+// tokens beside 13 decodes 46.5, 39.8 and 40.2; a chunk of 2048 tokens over 8192
+// keys 248 as it is (one piece) and 284 with twice as many. One decode over 8192
+// keys with pieces of 256 keys 12.6, of 128 14.2.
 void plan_attention(AttentionArgs* a) {
   const int64_t cus = device_cus(), rows = (int64_t)a->T * (a->G < kRows ? a->G : kRows);
   const bool all_few = rows <= (int64_t)kRows * a->N, all_tile = !all_few && a->N == 1;

@@ -215,6 +215,7 @@ struct AttentionArgs {
   void* out; int64_t o_t, o_h;
   float* part;       // [pieces, T, HQ, D] sums of p v, unnormalised
   float* part_ml;    // [pieces, T, HQ, 2] running maximum and sum
+  int32_t turn;      // tiles of one sequence: the first places on every compute unit (0: no matter)
   int32_t T, N, HQ, HKV, G, D, page, n_pages, max_context;
   // keys a workgroup walks and the most such pieces a context has, for the
   // sequences of few rows ([0], at most few_rows rows a key head) and the others ([1])

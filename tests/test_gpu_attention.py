@@ -315,3 +315,11 @@ def test_append_then_attend(device):
     a.update(positions=i32(pos, device), slot_mapping=i32(slot, device), k_cache=x["k_cache"], v_cache=x["v_cache"])
     x["q"] = check_append(a)
     check_attention(x)
+
+
+@pytest.mark.parametrize("new,context,heads,kv_heads,dim", [(1030, 1100, 16, 8, 64), (2500, 2500, 8, 1, 128), (1100, 1130, 32, 32, 64),
+                                                            (700, 720, 24, 8, 256)])
+def test_many_tiles_of_one_sequence(device, new, context, heads, kv_heads, dim):
+    """More tiles than compute units, and twice as many: every row once,
+    whatever the order that the tiles are taken in."""
+    check_attention(make_attention([new], [context], device, heads=heads, kv_heads=kv_heads, dim=dim, seed=new))
