@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
   __shared__ int bad_key;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int slot = blockIdx.x, h = blockIdx.y;
+  const int slot = blockIdx.x, h = blockIdx.y, g_first = 2 * blockIdx.z;
 
   // the slot's sequence and first row
   int n = -1;
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
   if (threadIdx.x == 0) bad_key = C;
 
   // every row's keys and queries, 16 lanes a row, and the gates of the first
-  // two value heads are asked for at once
+  // two of its value heads are asked for at once
   uint8_t* unit = w.unit + ((int64_t)slot * a.H + h) * unit_bytes(SPLIT);
   Raw<Act, 8> rows[8];
 #pragma unroll
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
     ga = Gate::ld(a.a, at * a.a_t + hv * a.a_h), gb = Gate::ld(a.bgate, at * a.bg_t + hv * a.bg_h);
     g_log = a.a_log[hv * a.al_s], g_bias = a.dt_bias[hv * a.db_s];
   };
-  load_gates(0);
+  load_gates(g_first);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -382,10 +382,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
     const Operand<SPLIT> o = operand<SPLIT>(f32x4_t{x[0] * f, x[1] * f, x[2] * f, x[3] * f}, f32x4_t{x[4] * f, x[5] * f, x[6] * f, x[7] * f});
     const int plane = (is_q ? P : 0);
     *(u32x4_t*)(lds + (plane * C + t) * RS + 16 * col) = o.hi;
+    if constexpr (SPLIT) *(u32x4_t*)(lds + ((plane + 1) * C + t) * RS + 16 * col) = o.lo;
+    if (g_first) continue;  // (the first workgroup of the group writes them)
     *(uint2*)(unit + plane * C * 2 * K + unit_at(t, 2 * col)) = make_uint2(o.hi[0], o.hi[1]);
     *(uint2*)(unit + plane * C * 2 * K + unit_at(t, 2 * col + 1)) = make_uint2(o.hi[2], o.hi[3]);
     if constexpr (SPLIT) {
-      *(u32x4_t*)(lds + ((plane + 1) * C + t) * RS + 16 * col) = o.lo;
       *(uint2*)(unit + (plane + 1) * C * 2 * K + unit_at(t, 2 * col)) = make_uint2(o.lo[0], o.lo[1]);
       *(uint2*)(unit + (plane + 1) * C * 2 * K + unit_at(t, 2 * col + 1)) = make_uint2(o.lo[2], o.lo[3]);
     }
@@ -414,14 +415,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
   }
 
   // the group's value heads, two at a time
-  for (int g0 = 0; g0 < a.G; g0 += 2) {
+  for (int g0 = g_first; g0 < a.G; g0 += 2 * gridDim.z) {
     const int heads = min(2, a.G - g0);
     __syncthreads();  // the units (or the last heads' M) are no longer read
     if (wave < heads) {
       const int hv = h * a.G + g0 + wave, t = lane;
       float g = 0.f, beta = 0.f;
       bool bad = t >= bad_key;
-      if (g0) load_gates(g0);
+      if (g0 != g_first) load_gates(g0);
       if (t < len) {
         g = log_decay(ga + g_bias, g_log);
         beta = sigmoid(gb);
@@ -1075,9 +1076,15 @@ bool needs_split(int act_dt, int state_dt) { return act_dt != DT_BF16 || state_d
 // and 29.
 bool chunked_form(int64_t T, int64_t N, bool split) { return T >= (split ? 32 : 16) * N; }
 
+// A workgroup takes a key head's value heads two after two; while that leaves
+// compute units idle each two have one of their own, which forms the keys' part
+// again (26 chunks of 4 key heads and 12 value heads, f16 with an f32 state: 20.5
+// us in one part, 16.5 in two).
 template <class Act, bool GATE_F32, bool SPLIT>
 int launch_prep(const PrefillArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((chunk_prep_kernel<Act, GATE_F32, SPLIT>), dim3(a.T / C + a.N, a.H), dim3(256), 0, s, a);
+  const int64_t chunks = a.T / C + a.N;
+  const uint32_t parts = chunks * a.H < device_cus() ? (a.G + 1) / 2 : 1;
+  hipLaunchKernelGGL((chunk_prep_kernel<Act, GATE_F32, SPLIT>), dim3((uint32_t)chunks, a.H, parts), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
 template <class Act, class St, bool SPLIT, int WAVES, bool ROLES>

@@ -318,3 +318,11 @@ def test_order_of_the_batch(device):
     y["slots"] = y["slots"][order]
     y["cu"] = torch.tensor(np.concatenate([[0], np.cumsum([lengths[i] for i in order])]), dtype=torch.int32, device=device)
     assert torch.equal(run(y), whole[at]) and torch.equal(y["state"], x["state"])
+
+
+@pytest.mark.parametrize("heads,value_heads", [(1, 3), (2, 10), (4, 16), (1, 32)])
+@pytest.mark.parametrize("act,state", [(BF16, BF16), (F16, F32)])
+def test_value_heads_in_parts(device, heads, value_heads, act, state):
+    """Few chunks of key heads with several value heads each: the preparation's
+    workgroups share a key head."""
+    check(make([70, 40], device, seed=value_heads, heads=heads, value_heads=value_heads, act=act, state=state))
