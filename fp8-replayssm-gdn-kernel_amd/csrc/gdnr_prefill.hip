@@ -598,20 +598,28 @@ __device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, 
   }
 }
 
-// The sequence at a place of the launch's order: of each 64, the longest first.
-// Workgroups start in order as others end, so that the last to start are then
-// short ones (24 sequences of up to 1096 tokens: the scan 186 us as given, 168 so).
+// The sequence at a place of the launch's order: of each 64, those of most chunks
+// first. Workgroups start in order as others end, so that the last to start are
+// then short ones (24 sequences of up to 1096 tokens: the scan 186 us as given,
+// 168 so). The place is looked for bit by bit of the chunk counts.
 __device__ __forceinline__ int longest_first(const PrefillArgs& a, int place) {
   const int lane = threadIdx.x & 63, base = place & ~63, count = min(64, a.N - base);
-  uint32_t key = 0;  // by length, then by index
+  uint32_t size = 0;
   if (lane < count) {
     const int64_t at = (base + lane) * a.cu_s;
     const int begin = min(max(a.cu[at], 0), a.T), end = min(max(a.cu[at + a.cu_s], begin), a.T);
-    key = (uint32_t)(end - begin) * 64 + 64 - lane;
+    size = (uint32_t)(end - begin + C - 1) / C;
   }
-  int longer = 0;
-  for (int j = 0; j < count; ++j) longer += __builtin_amdgcn_readlane(key, j) > key;
-  return __builtin_amdgcn_readfirstlane(base + __builtin_ctzll(__ballot(lane < count && longer == place - base)));
+  uint64_t left = __ballot(lane < count);
+  int k = place - base;  // the place among those left
+  for (int bit = 31 - __builtin_clz((uint32_t)(a.T / C + 1)); bit >= 0; --bit) {
+    const uint64_t set = __ballot(size >> bit & 1) & left;
+    const int larger = __popcll(set);
+    left &= k < larger ? set : ~set;
+    if (k >= larger) k -= larger;
+  }
+  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(left >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left, 0));
+  return __builtin_amdgcn_readfirstlane(base + __builtin_ctzll(__ballot((left >> lane & 1) && before == k)));
 }
 
 // LDS of the scan: a chunk's keys, scalars and T tiles twice (the next chunk's
@@ -1071,8 +1079,8 @@ bool needs_split(int act_dt, int state_dt) { return act_dt != DT_BF16 || state_d
 
 // The chunked form from an average of 16 tokens a sequence on (SPLIT: 32). us
 // a call, token by token and in chunks, HV=32, V=128, bf16: one sequence of 16
-// tokens 14.9 and 19.5, of 24 20.0 and 19.4; 64 sequences of 8 72 and 109, of 16
-// 125 and 110; f16 with an f32 state, 4 sequences of 32 25.6 and 29.0, of 64 46
+// tokens 14.9 and 17.5, of 24 20.0 and 17.0; 64 sequences of 8 72 and 109, of 16
+// 125 and 109; f16 with an f32 state, 4 sequences of 32 25.6 and 28.3, of 64 46
 // and 29.
 bool chunked_form(int64_t T, int64_t N, bool split) { return T >= (split ? 32 : 16) * N; }
 
