@@ -604,6 +604,7 @@ __device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, 
 // 168 so). The place is looked for bit by bit of the chunk counts.
 __device__ __forceinline__ int longest_first(const PrefillArgs& a, int place) {
   const int lane = threadIdx.x & 63, base = place & ~63, count = min(64, a.N - base);
+  if (count == 1) return base;
   uint32_t size = 0;
   if (lane < count) {
     const int64_t at = (base + lane) * a.cu_s;
@@ -1079,7 +1080,7 @@ bool needs_split(int act_dt, int state_dt) { return act_dt != DT_BF16 || state_d
 
 // The chunked form from an average of 16 tokens a sequence on (SPLIT: 32). us
 // a call, token by token and in chunks, HV=32, V=128, bf16: one sequence of 16
-// tokens 14.9 and 17.5, of 24 20.0 and 17.0; 64 sequences of 8 72 and 109, of 16
+// tokens 14.9 and 16.8, of 24 20.0 and 16.5; 64 sequences of 8 72 and 109, of 16
 // 125 and 109; f16 with an f32 state, 4 sequences of 32 25.6 and 28.3, of 64 46
 // and 29.
 bool chunked_form(int64_t T, int64_t N, bool split) { return T >= (split ? 32 : 16) * N; }
