@@ -1349,11 +1349,6 @@ int check_cache(const gdnr_tensor* c, const char* name, int act, int64_t heads, 
     return fail(GDNR_ERR_UNSUPPORTED, "%s: spans 2^36 bytes or more", name);
   return GDNR_OK;
 }
-
-int64_t attention_workspace(const gdnr::AttentionArgs& a) {
-  const int64_t pieces = std::max(a.pieces[0], a.pieces[1]);
-  return pieces > 1 ? pieces * a.T * a.HQ * (a.D + 2) * 4 : 0;
-}
 }  // namespace
 
 int64_t gdnr_prefill_workspace(int64_t tokens, int64_t sequences, int32_t heads, int32_t value_heads, int32_t value_dim,
@@ -1510,7 +1505,7 @@ int64_t gdnr_paged_attention_workspace(int64_t tokens, int64_t sequences, int32_
   a.T = (int32_t)tokens, a.N = (int32_t)sequences, a.HQ = heads, a.HKV = kv_heads, a.G = heads / kv_heads, a.D = head_dim;
   a.max_context = (int32_t)max_context;
   gdnr::plan_attention(&a);
-  return attention_workspace(a);
+  return gdnr::place_pieces(&a, nullptr);
 }
 
 int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const gdnr_tensor* v_cache,
@@ -1553,7 +1548,8 @@ int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const
   r.max_context = max_context;
   gdnr::plan_attention(&r);
   if (std::max(r.pieces[0], r.pieces[1]) > 65535) return fail(GDNR_ERR_UNSUPPORTED, "a context of %d keys has too many pieces", max_context);
-  GDNR_TRY(check_workspace(workspace, attention_workspace(r)));
+  GDNR_TRY(check_workspace(workspace, gdnr::place_pieces(&r, nullptr)));
+  if (workspace) gdnr::place_pieces(&r, (float*)workspace->data);
   r.q = q->data, r.q_t = q->strides[0], r.q_h = q->strides[1];
   r.k_cache = k_cache->data, r.kc_p = k_cache->strides[0], r.kc_t = k_cache->strides[1], r.kc_h = k_cache->strides[2];
   r.v_cache = v_cache->data, r.vc_p = v_cache->strides[0], r.vc_t = v_cache->strides[1], r.vc_h = v_cache->strides[2];
@@ -1561,10 +1557,6 @@ int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const
   r.cu = (const int32_t*)cu_seqlens->data, r.cu_s = cu_seqlens->strides[0];
   r.context = (const int32_t*)context_lens->data, r.cx_s = context_lens->strides[0];
   r.out = out->data, r.o_t = out->strides[0], r.o_h = out->strides[1];
-  if (const int64_t most = std::max(r.pieces[0], r.pieces[1]); most > 1) {
-    r.part = (float*)workspace->data;
-    r.part_ml = r.part + most * T * HQ * D;
-  }
   r.page = (int32_t)page, r.n_pages = (int32_t)pages;
   r.scale_log2 = scale * 1.4426950408889634f;
   return hip_status(gdnr::launch_attention(r, act, stream));

@@ -151,6 +151,10 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int n) {
 __device__ __forceinline__ bool few_rows(const AttentionArgs& a, const Span& s) {
   return (int64_t)(s.end - s.begin) * min(a.G, kRows) <= a.few_rows;
 }
+// place of token t among the pieces of its kind (0: few rows)
+__device__ __forceinline__ int64_t piece_row(const AttentionArgs& a, int kind, int n, const Span& s, int t) {
+  return kind == 0 && a.few_rows == kRows ? (int64_t)n * (kRows / min(a.G, kRows)) + (t - s.begin) : t;
+}
 // keys that token t of the sequence sees
 __device__ __forceinline__ int visible(const Span& s, int t) { return min(max(s.context - s.end + t + 1, 0), s.context); }
 
@@ -367,6 +371,7 @@ __device__ __forceinline__ void few_step(const AttentionArgs& a, uint8_t* lds, c
   }
   const int qh = hk * a.G + head;
   const float norm = pieces > 1 ? 1.f : visible(sq, t) == 0 ? 0.f : 1.f / l;
+  const int64_t part_at = (blk.z * a.part_rows[0] + piece_row(a, 0, n, sq, t)) * a.HQ + qh;
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) {
     const int d = 64 * i + 4 * dl;
@@ -375,13 +380,13 @@ __device__ __forceinline__ void few_step(const AttentionArgs& a, uint8_t* lds, c
     for (int w = 0; w < kWaves; ++w) sum += f[w] * *(const f32x4_t*)(lds + (w * kRows + row) * o_stride<D>() + 4 * d);
     sum *= norm;
     if (pieces > 1) {
-      *(f32x4_t*)(a.part + (((int64_t)blk.z * a.T + t) * a.HQ + qh) * D + d) = sum;
+      *(f32x4_t*)(a.part[0] + part_at * D + d) = sum;
     } else {
       *(uint2*)((uint8_t*)a.out + (t * a.o_t + qh * a.o_h + d) * 2) = make_uint2(pack2<Act>(sum[0], sum[1]), pack2<Act>(sum[2], sum[3]));
     }
   }
   if (pieces > 1 && dl == 0) {
-    float* p = a.part_ml + (((int64_t)blk.z * a.T + t) * a.HQ + qh) * 2;
+    float* p = a.part_ml[0] + part_at * 2;
     p[0] = top, p[1] = l;
   }
 }
@@ -678,10 +683,10 @@ __device__ __forceinline__ void tile_step(const AttentionArgs& a, uint8_t* lds, 
     if (!live[nt]) continue;
     const int qh = hk * a.G + rh[nt];
     if (pieces > 1) {
-      const int64_t at = ((int64_t)blk.z * a.T + rt[nt]) * a.HQ + qh;
+      const int64_t at = (blk.z * a.part_rows[1] + piece_row(a, 1, n, sq, rt[nt])) * a.HQ + qh;
 #pragma unroll
-      for (int i = 0; i < DT; ++i) *(f32x4_t*)(a.part + at * D + 16 * i + 4 * grp) = o[nt][i];
-      if (grp == 0) a.part_ml[2 * at] = m_run[nt], a.part_ml[2 * at + 1] = l;
+      for (int i = 0; i < DT; ++i) *(f32x4_t*)(a.part[1] + at * D + 16 * i + 4 * grp) = o[nt][i];
+      if (grp == 0) a.part_ml[1][2 * at] = m_run[nt], a.part_ml[1][2 * at + 1] = l;
     } else {
       const float norm = vis[nt] == 0 ? 0.f : 1.f / l;
       uint8_t* p = (uint8_t*)a.out + (rt[nt] * a.o_t + qh * a.o_h + 4 * grp) * 2;
@@ -731,14 +736,14 @@ __global__ __launch_bounds__(256) void join_kernel(const AttentionArgs a) {
   constexpr int W = D / 4, R = 64 / W, BATCH = 16;  // lanes a row, rows a wave, pieces in flight
   const int lane = threadIdx.x & 63, l = lane % W, t = blockIdx.x;
   const int h_own = (int)(blockIdx.y * 4 + (threadIdx.x >> 6)) * R + lane / W, h = min(h_own, a.HQ - 1);
-  const int64_t row0 = (int64_t)t * a.HQ + h, step = (int64_t)a.T * a.HQ;
-  const float* ml0 = a.part_ml + 2 * row0;
-  const float* p0 = a.part + row0 * D + 4 * l;
   const int n = sequences_up_to(a, t, 1, 0) - 1;
   if (n < 0) return;
   const Span sq = span_of(a, n);
   const int kind = few_rows(a, sq) ? 0 : 1, piece = a.piece[kind];
-  if (t >= sq.end || a.pieces[kind] == 1) return;
+  if (t < sq.begin || t >= sq.end || a.pieces[kind] == 1) return;
+  const int64_t row0 = piece_row(a, kind, n, sq, t) * a.HQ + h, step = a.part_rows[kind] * a.HQ;
+  const float* ml0 = a.part_ml[kind] + 2 * row0;
+  const float* p0 = a.part[kind] + row0 * D + 4 * l;
   const int vis = visible(sq, t), pieces = (vis + piece - 1) / piece;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   float top = -__builtin_inff(), sum = 0.f;
@@ -849,6 +854,24 @@ void plan_attention(AttentionArgs* a) {
   a->pieces[0] = a->pieces[1] = 0;
   if (!all_tile) plan(0, all_few && a->T > a->N ? tiles_of(kRows) : (int64_t)a->N * ((a->G + kRows - 1) / kRows), 8 * cus);
   if (!all_few) plan(1, tiles_of(a->D == 256 ? 64 : 128), 2 * cus);
+}
+
+// The kinds' pieces one after the other, then their maxima and sums. Where both
+// kinds occur, the sequences of few rows have one tile of tokens each (their
+// number of pieces goes by the number of sequences: it would be charged to every
+// token of a prompt beside them). A kind in one piece takes nothing.
+int64_t place_pieces(AttentionArgs* a, float* work) {
+  int64_t rows[2];
+  for (int kind = 0; kind < 2; ++kind) {
+    const bool by_sequence = kind == 0 && a->few_rows == kRows;
+    a->part_rows[kind] = by_sequence ? (int64_t)a->N * (kRows / (a->G < kRows ? a->G : kRows)) : a->T;
+    rows[kind] = a->pieces[kind] > 1 ? a->pieces[kind] * a->part_rows[kind] * a->HQ : 0;
+  }
+  if (work) {
+    a->part[0] = work, a->part[1] = work + rows[0] * a->D;
+    a->part_ml[0] = a->part[1] + rows[1] * a->D, a->part_ml[1] = a->part_ml[0] + 2 * rows[0];
+  }
+  return (rows[0] + rows[1]) * (a->D + 2) * 4;
 }
 
 int launch_attention(const AttentionArgs& a, int act_dt, void* stream) {

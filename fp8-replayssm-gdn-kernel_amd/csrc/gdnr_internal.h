@@ -213,8 +213,11 @@ struct AttentionArgs {
   const int32_t* cu; int64_t cu_s;
   const int32_t* context; int64_t cx_s;
   void* out; int64_t o_t, o_h;
-  float* part;       // [pieces, T, HQ, D] sums of p v, unnormalised
-  float* part_ml;    // [pieces, T, HQ, 2] running maximum and sum
+  // pieces of rows, for the sequences of few rows ([0]) and the others ([1]):
+  // sums of p v, unnormalised, [pieces, part_rows, HQ, D], and running maximum
+  // and sum, [pieces, part_rows, HQ, 2]
+  float* part[2]; float* part_ml[2];
+  int64_t part_rows[2];   // tokens that have a place there
   int32_t turn;      // tiles of one sequence: the first places on every compute unit (0: no matter)
   int32_t T, N, HQ, HKV, G, D, page, n_pages, max_context;
   // keys a workgroup walks and the most such pieces a context has, for the
@@ -269,6 +272,8 @@ int64_t prefill_work_bytes(int64_t T, int64_t N, int32_t H, int32_t HV, int act_
 int launch_prefill(const PrefillArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream);
 int launch_append(const AppendArgs& a, int act_dt, void* stream);
 void plan_attention(AttentionArgs* a);
+// Places the pieces in `work` from its start on; returns the bytes that they take
+int64_t place_pieces(AttentionArgs* a, float* work);
 int launch_attention(const AttentionArgs& a, int act_dt, void* stream);
 int launch_format_quantize(const FormatArgs& a, void* stream);
 int launch_format_dequantize(const FormatArgs& a, void* stream);

@@ -323,3 +323,19 @@ def test_many_tiles_of_one_sequence(device, new, context, heads, kv_heads, dim):
     """More tiles than compute units, and twice as many: every row once,
     whatever the order that the tiles are taken in."""
     check_attention(make_attention([new], [context], device, heads=heads, kv_heads=kv_heads, dim=dim, seed=new))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (6, 2, 64), (40, 2, 64), (16, 2, 256)])
+@pytest.mark.parametrize("new,contexts", [([1, 1, 300], [5000, 700, 900]), ([2, 600, 0, 1], [4000, 650, 0, 3]),
+                                          ([90, 1], [3000, 6000])])
+def test_pieces_of_either_kind(device, heads, kv_heads, dim, new, contexts):
+    """Decodes beside a prompt's chunk, each kind in its own number of pieces:
+    every piece lies inside the workspace that was asked for, and nothing that
+    the workspace held before is read."""
+    x = make_attention(new, contexts, device, heads=heads, kv_heads=kv_heads, dim=dim, seed=dim + sum(new))
+    most = max(contexts)
+    size = gdnr_lib.paged_attention_workspace(sum(new), len(new), heads, kv_heads, dim, most)
+    assert size > 0
+    workspace = torch.full((size + 4096,), 0xFF, dtype=torch.uint8, device=device)  # (NaN)
+    check_attention(x, max_context=most, workspace=workspace[:size])
+    assert (workspace[size:] == 0xFF).all()

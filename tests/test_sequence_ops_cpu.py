@@ -253,3 +253,24 @@ def test_oracle_attention_on_one_page_is_softmax():
         for h in range(2):
             p = np.exp(q[t, h] @ k[0, :3 + t, 0].T * 8 ** -0.5)
             assert np.abs(out[t, h] - p @ v[0, :3 + t, 0] / p.sum()).max() < 1e-12
+
+
+@pytest.mark.parametrize("prompt", [1024, 8192])
+@pytest.mark.parametrize("decodes", [1, 3, 40])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (64, 8, 256), (16, 2, 256), (8, 8, 64), (40, 2, 128)])
+@pytest.mark.parametrize("context", [12000, 131072])
+def test_mixed_batches_take_little_workspace(prompt, decodes, heads, kv_heads, dim, context):
+    """A few decodes beside a prompt's chunk. Eight workgroups of 16 rows a
+    compute unit hold the decodes' pieces and two of at most 128 the prompt's;
+    rounding pieces up, and rows of a tile that are no token's, at most double
+    either. 256 compute units; 4 (dim + 2) bytes a row."""
+    size = gdnr_lib.paged_attention_workspace(prompt + decodes, decodes + 1, heads, kv_heads, dim, context)
+    rows = 2 * (8 * 256 * 16 + 2 * 256 * 128)
+    assert size <= rows * 4 * (dim + 2)
+
+
+def test_a_prompt_in_one_piece_takes_none_beside_a_decode():
+    """The decodes' pieces alone: at most eight workgroups of 16 rows a compute unit, rounded up."""
+    assert gdnr_lib.paged_attention_workspace(8192, 1, 32, 8, 128, 131072) == 0
+    size = gdnr_lib.paged_attention_workspace(8193, 2, 32, 8, 128, 131072)
+    assert 0 < size <= 2 * 8 * 256 * 16 * 4 * (128 + 2)
