@@ -5,7 +5,7 @@
 // a row that sees no key gives 0. Heads are grouped: query head h reads the
 // keys of head h / G.
 //
-// One pass over the keys with a running maximum and sum (f32). The rows of a
+// One pass over the keys with a running reference near the maximum and sums (f32). The rows of a
 // workgroup are the (token, query head of the group) pairs of one key head, so
 // the keys of a group are read once. The scores are formed transposed,
 // K (keys x D) by Q^T: a lane then holds 8 keys of one row, which is, as it
@@ -68,6 +68,35 @@ __device__ __forceinline__ u32x4_t ones() {
 // each 16-lane group receives column i of the group's 4 rows
 __device__ __forceinline__ uint2 transposed4(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+}
+// A weight is 2^(score - reference). f16 has all its bits down to 2^-14 alone,
+// and a long tail of small weights under one large key is what the output consists of
+// where that key's value is 0: there the reference lies kHead below the
+// maximum that it was taken from, so that a weight that is 2^-27 of the largest keeps
+// all its bits and one of 2^-38 still counts. kLag: how far tile_kernel's scores
+// may pass that maximum before the reference follows; 2^(kHead + kLag + 1/2) fits
+// the type. (With a lag of 8 and no head, 18000 keys 18 below one whose value is 0 were
+// off by 0.2%; f16 rounds to 0.02%.) bf16 has f32's exponents.
+template <class Act>
+constexpr bool is_f16() { return !std::is_same<Act, ActBF16>::value; }
+template <class Act>
+constexpr float kHead = is_f16<Act>() ? 13.f : 0.f;
+template <class Act>
+constexpr float kLag = is_f16<Act>() ? 2.f : 8.f;
+// whether a maximum has passed the reference's own by more than lag (a
+// difference: exact where they are large)
+template <class Act>
+__device__ __forceinline__ bool passed(float top, float reference, float lag) {
+  if constexpr (is_f16<Act>()) return top - reference > kHead<Act> + lag;
+  else return top > reference + lag;
+}
+// the reference of a maximum (where top is so large that its neighbours are
+// further apart than that: itself)
+template <class Act>
+__device__ __forceinline__ float reference(float top) {
+  if constexpr (!is_f16<Act>()) return top;
+  const float r = top - kHead<Act>;
+  return top - r > kHead<Act> + 0.5f ? top : r;
 }
 // whether any of 8 values is an infinity or a NaN
 template <class Act>
@@ -252,7 +281,7 @@ __device__ __forceinline__ void few_step(const AttentionArgs& a, uint8_t* lds, c
   f32x4_t o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m_run = -__builtin_inff();
+  float m_run = -__builtin_inff();         // the reference
   f32x4_t l_run = {0.f, 0.f, 0.f, 0.f};  // (every row of it)
   constexpr int STEP = kWaves * kKeys;
   int key0 = k_begin + wave * kKeys;
@@ -284,8 +313,8 @@ __device__ __forceinline__ void few_step(const AttentionArgs& a, uint8_t* lds, c
       top = fmaxf(top, x[e]);
     }
     top = column_max(top);
-    if (__any(top > m_run)) {
-      const float m_new = fmaxf(m_run, top);
+    if (__any(passed<Act>(top, m_run, 0.f))) {
+      const float m_new = fmaxf(m_run, reference<Act>(top));
       const float f = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
       scale_in_place(l_run, f);
 #pragma unroll
@@ -495,7 +524,7 @@ __device__ __forceinline__ void tile_step(const AttentionArgs& a, uint8_t* lds, 
 
   f32x4_t o[NT][DT];
   f32x4_t l_run[NT];  // (every row of it)
-  float m_run[NT];
+  float m_run[NT];  // the references
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m_run[nt] = -__builtin_inff(), l_run[nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -581,8 +610,9 @@ __device__ __forceinline__ void tile_step(const AttentionArgs& a, uint8_t* lds, 
           for (int j = 0; j < 4; ++j)
             if (key0 + 16 * m + 4 * grp + j >= vis[nt]) s[m][nt][j] = -__builtin_inff();
     }
-    // The maximum follows the scores only when it falls 2^8 behind them: a
-    // weight then grows to 256 at most, and the outputs are rarely rescaled.
+    // The reference follows the scores only when their maximum has passed its
+    // own by kLag: a weight then grows by 2^kLag at most, and the outputs are
+    // rarely rescaled.
     float top[NT];
     bool behind = false;
 #pragma unroll
@@ -593,12 +623,12 @@ __device__ __forceinline__ void tile_step(const AttentionArgs& a, uint8_t* lds, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) top[nt] = fmaxf(top[nt], s[m][nt][j]);
       top[nt] = column_max(top[nt]);
-      behind |= top[nt] * scale > m_run[nt] + 8.f;
+      behind |= passed<Act>(top[nt] * scale, m_run[nt], kLag<Act>);
     }
     if (__any(behind)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float m_new = fmaxf(m_run[nt], top[nt] * scale);
+        const float m_new = fmaxf(m_run[nt], reference<Act>(top[nt] * scale));
         const float f = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m_run[nt] - m_new);
         scale_in_place(l_run[nt], f);
 #pragma unroll

@@ -214,8 +214,8 @@ struct AttentionArgs {
   const int32_t* context; int64_t cx_s;
   void* out; int64_t o_t, o_h;
   // pieces of rows, for the sequences of few rows ([0]) and the others ([1]):
-  // sums of p v, unnormalised, [pieces, part_rows, HQ, D], and running maximum
-  // and sum, [pieces, part_rows, HQ, 2]
+  // sums of p v, unnormalised, [pieces, part_rows, HQ, D], and reference
+  // and sum of weights, [pieces, part_rows, HQ, 2]
   float* part[2]; float* part_ml[2];
   int64_t part_rows[2];   // tokens that have a place there
   int32_t turn;      // tiles of one sequence: the first places on every compute unit (0: no matter)

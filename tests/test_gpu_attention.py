@@ -339,3 +339,32 @@ def test_pieces_of_either_kind(device, heads, kv_heads, dim, new, contexts):
     workspace = torch.full((size + 4096,), 0xFF, dtype=torch.uint8, device=device)  # (NaN)
     check_attention(x, max_context=most, workspace=workspace[:size])
     assert (workspace[size:] == 0xFF).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("gap", [12.0, 18.0])
+@pytest.mark.parametrize("new,contexts", [([1], [20000]), ([1, 1, 3], [6000, 3000, 4000]), ([300], [5000]), ([1, 100], [9000, 5000])])
+def test_tail_under_a_dominant_key(device, new, contexts, dim, gap, dtype):
+    """A key ahead of thousands of others by 12 or 18 (e^18 = 2^26), its value
+    0: the output is the others' sum, whose weights keep their bits. (Values of
+    some 2^12, so that such a sum is no subnormal number of f16's.)"""
+    x = make_attention(new, contexts, device, dim=dim, dtype=dtype, seed=dim, spread=1.0)
+    x["v_cache"] *= 4096
+    u = torch.full((dim,), dim ** -0.5, device=device)
+    q = x["q"].float()
+    x["q"] = (q - (q @ u)[..., None] * u + 8 * u).to(dtype)
+    for n in range(len(new)):
+        at = int(x["block_table"][n, 0]), 5
+        x["k_cache"][at] = (gap * dim ** 0.5 / 8 * u).to(dtype)
+        x["v_cache"][at] = 0
+    check_attention(x)
+
+
+@pytest.mark.parametrize("scale", [1.0, 60.0, 8000.0])
+def test_large_scores_in_f16(device, scale):
+    """Scores of a few units, of 1e4 and of 2^27, where floats are 8 apart."""
+    x = make_attention([1, 40, 2], [3000, 700, 50], device, dtype=F16, seed=21)
+    x["q"] *= scale
+    x["k_cache"] *= scale
+    check_attention(x)
