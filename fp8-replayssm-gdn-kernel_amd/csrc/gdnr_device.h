@@ -301,6 +301,24 @@ __device__ __forceinline__ bool wait_count(int* f, int target, uint32_t* status,
   return false;
 }
 
+// ---------------------------------------------------------------- norms of rows
+// A row that is normed lies in LANES consecutive lanes, 8 elements each. Where a
+// lane's sum of squares reaches kLargeSquares (f32 or bf16 rows of 2^28 and more: the
+// row's own may pass f32's range) the row is taken times row_factor first, a power of
+// two that brings its largest element to [2^20, 2^21): 1 where that is below
+// 2^28 or not finite.
+constexpr float kLargeSquares = 0x1p60f;
+template <int LANES>
+__device__ __forceinline__ float row_factor(const float (&x)[8]) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  const uint32_t exponent = __float_as_uint(top) >> 23;
+  return exponent >= 155 && exponent < 255 ? __uint_as_float((274 - exponent) << 23) : 1.f;
+}
+
 // ---------------------------------------------------------------- global -> LDS
 // Direct global -> LDS copy of 16 bytes per lane (global_load_lds_dwordx4):
 // lane l's 16 bytes land at LDS address lds_addr + 16 l (lds_addr wave-uniform,

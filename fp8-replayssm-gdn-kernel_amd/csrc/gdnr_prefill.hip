@@ -26,6 +26,10 @@ __device__ __forceinline__ float sum16(float x) {
   return x + dpp_f<kDppMirror>(x);
 }
 
+// whether the squares of a key or query may pass f32's range
+template <class Act>
+constexpr bool kMayBeLarge = !std::is_same<Act, ActF16>::value;
+
 // N consecutive elements at p (N * kBytes a multiple of 8, p aligned to it up
 // to 16) as raw words, and their values
 template <class Act, int N>
@@ -136,6 +140,19 @@ __global__ __launch_bounds__(256) void recurrent_kernel(const PrefillArgs a) {
       qq = fmaf(qf[e], qf[e], qq);
       kk = fmaf(kf[e], kf[e], kk);
       qk = fmaf(qf[e], kf[e], qk);
+    }
+    if constexpr (kMayBeLarge<Act>) {
+      if (__any(fmaxf(qq, kk) >= kLargeSquares)) {
+        const float fq = row_factor<16>(qf), fk = row_factor<16>(kf);
+        qq = 0.f, kk = 0.f, qk = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          qf[e] *= fq, kf[e] *= fk;
+          qq = fmaf(qf[e], qf[e], qq);
+          kk = fmaf(kf[e], kf[e], kk);
+          qk = fmaf(qf[e], kf[e], qk);
+        }
+      }
     }
     const float rq = __builtin_amdgcn_rsqf(sum16(qq) + 1e-6f), rk = __builtin_amdgcn_rsqf(sum16(kk) + 1e-6f);
     const float gamma = readlane_f(gamma64, (t - begin) & 63), beta = readlane_f(beta64, (t - begin) & 63);
@@ -370,6 +387,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
     float x[8], ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = t < len ? rows[i][e] : 0.f, ss = fmaf(x[e], x[e], ss);
+    if constexpr (kMayBeLarge<Act>) {
+      if (__any(ss >= kLargeSquares)) {
+        const float f = row_factor<16>(x);
+        ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= f, ss = fmaf(x[e], x[e], ss);
+      }
+    }
     ss = sum16(ss);
     float f = __builtin_amdgcn_rsqf(ss + 1e-6f);
     if (!is_q && !(ss < __builtin_inff())) {

@@ -326,3 +326,15 @@ def test_value_heads_in_parts(device, heads, value_heads, act, state):
     """Few chunks of key heads with several value heads each: the preparation's
     workgroups share a key head."""
     check(make([70, 40], device, seed=value_heads, heads=heads, value_heads=value_heads, act=act, state=state))
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("lengths", [[9], [100]])
+@pytest.mark.parametrize("magnitude", [1e8, 1e18, 1e20, 1e30, 5e37])
+def test_large_keys_and_queries(device, lengths, act, magnitude):
+    """Keys and queries whose squares leave f32: their unit rows are what they
+    are at any magnitude, some rows large and some not."""
+    x = make(lengths, device, seed=41, act=act, state=act)
+    x["mixed"][::2, :512] *= magnitude
+    x["mixed"][1::4, :256] *= magnitude  # (queries alone)
+    check(x)
