@@ -160,7 +160,16 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
           if (weight) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) sq = fmaf(x[e], x[e], sq);
-            r = 1.f / sqrtf(group_sum<LPH>(sq) * (1.f / D) + a.eps);
+            float eps = a.eps;
+            if constexpr (std::is_same<Act, ActBF16>::value) {  // (f16's squares stay in range)
+              if (__any(sq >= kLargeSquares)) {
+                const float f = row_factor<LPH>(x);
+                sq = 0.f, eps *= f * f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= f, z[e] *= f, sq = fmaf(x[e], x[e], sq);
+              }
+            }
+            r = 1.f / sqrtf(group_sum<LPH>(sq) * (1.f / D) + eps);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= cw[e];

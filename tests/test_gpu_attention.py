@@ -368,3 +368,16 @@ def test_large_scores_in_f16(device, scale):
     x["q"] *= scale
     x["k_cache"] *= scale
     check_attention(x)
+
+
+@pytest.mark.parametrize("dim,rotary", [(64, 32), (128, 128), (256, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("magnitude", [1e8, 1e18, 1e20, 1e30, 5e37])
+def test_append_large_rows(device, dim, rotary, interleaved, magnitude):
+    """Heads whose squares leave f32 are normed like any others, beside some
+    that are not large and under a large eps too."""
+    x = make_append(40, device, heads=6, kv_heads=2, dim=dim, rotary=rotary, seed=22)
+    x["q"][::2] *= magnitude
+    x["k"][1::3, 0] *= magnitude
+    check_append(x, interleaved=interleaved)
+    check_append(x, interleaved=interleaved, eps=1e10)
