@@ -181,6 +181,7 @@ struct PrefillArgs {
   const uint8_t* started; int64_t sd_s;  // nullptr: every sequence continues from its slot's state
   void* out; int64_t o_t, o_h;
   int32_t T, N, H, HV, V, G;
+  int32_t chunk_from;  // tokens from which on a sequence is walked in chunks (0: each is)
   float out_scale;
   uint8_t* work;  // chunked form: what prefill_work_bytes counts
 };

@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256) void recurrent_kernel(const PrefillArgs a) {
   int begin, end;
   sequence_rows(a, n, begin, end);
   const bool started = sequence_started(a, n);
-  if (begin == end && started) return;
+  if ((begin == end && started) || end - begin >= a.chunk_from) return;
   uint8_t* sp = (uint8_t*)a.state + ((int64_t)sequence_slot(a, n) * a.st_s + hv * a.st_h + (int64_t)(row0 + 4 * grp) * a.st_v + 8 * cl) * St::kBytes;
   const int64_t srow = a.st_v * St::kBytes;
   float S[4][8];
@@ -267,21 +267,47 @@ __device__ __forceinline__ f32x4_t product(const Operand<SPLIT>& a, const Operan
 // (SPLIT: high, then low), a row's pieces as unit_at places them; per slot and
 // value head the tokens' {beta}[C], {-beta e^G}[C], {e^(G_C - G)}[C], {e^G}[C],
 // first bad token (an int), padded to 2 KiB, then the operand tiles of T - I and
-// of A (64 lanes x 16 bytes each; SPLIT: high, then low). Sequence n's chunks take
-// the slots from cu[n] / C + n on.
+// of A (64 lanes x 16 bytes each; SPLIT: high, then low). The chunks
+// of a sequence take slots one after the other.
 constexpr int kScalars = 2048;
 __host__ __device__ constexpr int64_t plane_bytes(bool split) { return C * K * 2 * (split ? 2 : 1); }  // keys, or queries
 __host__ __device__ constexpr int64_t unit_bytes(bool split) { return 2 * plane_bytes(split); }
 __host__ __device__ constexpr int64_t tri_bytes(bool split) { return kTri * 1024 * (split ? 2 : 1); }
 __host__ __device__ constexpr int64_t head_bytes(bool split) { return kScalars + 2 * tri_bytes(split); }
 
+// One of 64 sequences n, a lane's, among them (a.N and more: none): its tokens,
+// whether it is walked in chunks, and how many before it and in all of the 64 are.
+struct Lengths {
+  int begin, end, chunked_before, chunked_all;
+  bool chunked;
+};
+__device__ __forceinline__ Lengths lengths_of(const PrefillArgs& a, int n) {
+  Lengths x = {0, 0, 0, 0, false};
+  if (n < a.N) {
+    x.begin = min(max(a.cu[n * a.cu_s], 0), a.T), x.end = min(max(a.cu[(n + 1) * a.cu_s], x.begin), a.T);
+    x.chunked = x.end - x.begin >= a.chunk_from;
+  }
+  const uint64_t m = __ballot(x.chunked);
+  x.chunked_before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  x.chunked_all = __popcll(m);
+  return x;
+}
+// most sequences that may be walked in chunks
+__host__ __device__ inline int64_t chunked_most(int64_t T, int64_t N, int32_t chunk_from) {
+  return chunk_from && T / chunk_from < N ? T / chunk_from : N;
+}
+// slots of chunks: sequence n's are those from begin / C + the sequences in chunks
+// before it on
+__host__ __device__ inline int64_t chunk_slots(int64_t T, int64_t N, int32_t chunk_from) {
+  return T / C + chunked_most(T, N, chunk_from);
+}
+
 struct Work {
   uint8_t* unit;  // [slots][H]
   uint8_t* head;  // [slots][HV]
 };
 __host__ __device__ inline Work work_of(const PrefillArgs& a, bool split) {
-  const int64_t slots = a.T / C + a.N;
-  return {a.work, a.work + slots * a.H * unit_bytes(split)};
+  return {a.work, a.work + chunk_slots(a.T, a.N, a.chunk_from) * a.H * unit_bytes(split)};
 }
 
 // Byte of 4 elements (k = 4 k4 ..) of row t. A 16-byte piece holds the 8 elements
@@ -348,16 +374,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
   const int slot = blockIdx.x, h = blockIdx.y, g_first = 2 * blockIdx.z;
 
   // the slot's sequence and first row
-  int n = -1;
+  int n = -1, first_slot = 0, before = 0;
   for (int n0 = 0; n0 < a.N; n0 += 64) {
-    bool below = false;
-    if (n0 + lane < a.N) below = min(max(a.cu[(n0 + lane) * a.cu_s], 0), a.T) / C + n0 + lane <= slot;
-    n += __popcll(__ballot(below));
+    const Lengths own = lengths_of(a, n0 + lane);
+    const int from = own.begin / C + before + own.chunked_before;
+    const uint64_t at = __ballot(own.chunked && from <= slot);
+    if (at) {
+      n = n0 + 63 - __builtin_clzll(at);
+      first_slot = __builtin_amdgcn_readlane(from, 63 - __builtin_clzll(at));
+    }
+    before += own.chunked_all;
   }
   if (n < 0) return;
   int begin, end;
   sequence_rows(a, n, begin, end);
-  const int row0 = begin + (slot - begin / C - n) * C, len = min(end - row0, C);
+  const int row0 = begin + (slot - first_slot) * C, len = min(end - row0, C);
   if (len <= 0) return;
   const Work w = work_of(a, SPLIT);
   if (threadIdx.x == 0) bad_key = C;
@@ -623,29 +654,33 @@ __device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, 
   }
 }
 
-// The sequence at a place of the launch's order: of each 64, those of most chunks
-// first. Workgroups start in order as others end, so that the last to start are
+// The sequence at a place of the launch's order (-1: none) and its first slot: of each
+// 64 sequences those of most chunks first. Workgroups start in order as others end, so that the last to start are
 // then short ones (24 sequences of up to 1096 tokens: the scan 186 us as given,
 // 168 so). The place is looked for bit by bit of the chunk counts.
-__device__ __forceinline__ int longest_first(const PrefillArgs& a, int place) {
-  const int lane = threadIdx.x & 63, base = place & ~63, count = min(64, a.N - base);
-  if (count == 1) return base;
-  uint32_t size = 0;
-  if (lane < count) {
-    const int64_t at = (base + lane) * a.cu_s;
-    const int begin = min(max(a.cu[at], 0), a.T), end = min(max(a.cu[at + a.cu_s], begin), a.T);
-    size = (uint32_t)(end - begin + C - 1) / C;
-  }
-  uint64_t left = __ballot(lane < count);
-  int k = place - base;  // the place among those left
+__device__ __forceinline__ int longest_first(const PrefillArgs& a, int place, int& first_slot) {
+  const int lane = threadIdx.x & 63, most = min((int)chunked_most(a.T, a.N, a.chunk_from), 64), group = place / most, base = 64 * group;
+  first_slot = 0;
+  if (a.N == 1) return 0;  // (in chunks)
+  int before = 0;
+  if (a.chunk_from == 0) before = base;
+  else
+    for (int n0 = 0; n0 < base; n0 += 64) before += lengths_of(a, n0 + lane).chunked_all;
+  const Lengths own = lengths_of(a, base + lane);
+  const uint32_t size = (uint32_t)(own.end - own.begin + C - 1) / C;
+  uint64_t left = __ballot(own.chunked);
+  int k = place - group * most;  // the place among those left
+  if (k >= own.chunked_all) return -1;
   for (int bit = 31 - __builtin_clz((uint32_t)(a.T / C + 1)); bit >= 0; --bit) {
     const uint64_t set = __ballot(size >> bit & 1) & left;
     const int larger = __popcll(set);
     left &= k < larger ? set : ~set;
     if (k >= larger) k -= larger;
   }
-  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(left >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left, 0));
-  return __builtin_amdgcn_readfirstlane(base + __builtin_ctzll(__ballot((left >> lane & 1) && before == k)));
+  const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(left >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left, 0));
+  const int at = __builtin_ctzll(__ballot((left >> lane & 1) && rank == k));
+  first_slot = __builtin_amdgcn_readlane(own.begin / C + before + own.chunked_before, at);
+  return __builtin_amdgcn_readfirstlane(base + at);
 }
 
 // LDS of the scan: a chunk's keys, scalars and T tiles twice (the next chunk's
@@ -695,7 +730,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   const bool chain = !ROLES || wave == 0, outputs = !ROLES || wave == 1, fetches = !ROLES || wave == 2;
   // Workgroups go to the 8 XCDs in turn: those of one key head, which read the
   // same keys and queries, to one of them.
-  const int blocks = a.V / COLS, n = longest_first(a, blockIdx.y);
+  int first_slot;
+  const int blocks = a.V / COLS, n = longest_first(a, blockIdx.y, first_slot);
+  if (n < 0) return;
   int unit_id = blockIdx.x;
   if (a.H % 8 == 0) {
     const int per = a.G * blocks, j = unit_id >> 3;
@@ -708,11 +745,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   const bool started = sequence_started(a, n);
   if (begin == end && started) return;
   const int len = end - begin, chunks = (len + C - 1) / C;
+  const int64_t slot0 = a.N == 1 ? begin / C : first_slot;
+  if (slot0 + chunks > chunk_slots(a.T, a.N, a.chunk_from)) return;  // (offsets that decrease)
   const uint8_t *unit, *head;  // of chunk 0
   const int64_t unit_step = a.H * unit_bytes(SPLIT), head_step = a.HV * head_bytes(SPLIT);
   {
     const Work w = work_of(a, SPLIT);
-    const int64_t slot0 = begin / C + n;
     unit = w.unit + slot0 * unit_step + h * unit_bytes(SPLIT);
     head = w.head + slot0 * head_step + hv * head_bytes(SPLIT);
   }
@@ -1103,12 +1141,22 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 // Whether results keep more than bf16 does.
 bool needs_split(int act_dt, int state_dt) { return act_dt != DT_BF16 || state_dt != DT_BF16; }
 
-// The chunked form from an average of 16 tokens a sequence on (SPLIT: 32). us
-// a call, token by token and in chunks, HV=32, V=128, bf16: one sequence of 16
-// tokens 14.9 and 16.8, of 24 20.0 and 16.5; 64 sequences of 8 72 and 109, of 16
-// 125 and 109; f16 with an f32 state, 4 sequences of 32 25.6 and 28.3, of 64 46
-// and 29.
-bool chunked_form(int64_t T, int64_t N, bool split) { return T >= (split ? 32 : 16) * N; }
+// Which sequences are walked in chunks (PrefillArgs::chunk_from). The host knows
+// their number and the sum of their tokens. All of them from an average of 16
+// tokens a sequence on (SPLIT: 32). us a call, token by token and in chunks, HV=32,
+// V=128, bf16: one sequence of 16 tokens 14.9 and 16.8, of 24 20.0 and 16.5; 64
+// sequences of 8 72 and 109, of 16 125 and 109; f16 with an f32 state, 4 sequences of
+// 32 25.6 and 28.3, of 64 46 and 29. Below that a batch may still hold a long one
+// beside many short: from kLongWalk tokens in all, those of a chunk and more are
+// walked in chunks and the others token by token. us a call, all token by token and
+// so, bf16: 900 tokens beside 63 single ones 598 and 104, 120 beside 15 85 and 31;
+// where none is long the kernels with nothing to do cost 4: 16 sequences of 12
+// tokens 29 and 33, 64 of 8 70 and 72.
+constexpr int kLongWalk = 128;
+int32_t chunk_start(int64_t T, int64_t N, bool split) {
+  if (T >= (split ? 32 : 16) * N) return 0;
+  return T >= kLongWalk ? C : INT32_MAX;
+}
 
 // A workgroup takes a key head's value heads two after two; while that leaves
 // compute units idle each two have one of their own, which forms the keys' part
@@ -1116,10 +1164,15 @@ bool chunked_form(int64_t T, int64_t N, bool split) { return T >= (split ? 32 : 
 // us in one part, 16.5 in two).
 template <class Act, bool GATE_F32, bool SPLIT>
 int launch_prep(const PrefillArgs& a, hipStream_t s) {
-  const int64_t chunks = a.T / C + a.N;
+  const int64_t chunks = chunk_slots(a.T, a.N, a.chunk_from);
   const uint32_t parts = chunks * a.H < device_cus() ? (a.G + 1) / 2 : 1;
   hipLaunchKernelGGL((chunk_prep_kernel<Act, GATE_F32, SPLIT>), dim3((uint32_t)chunks, a.H, parts), dim3(256), 0, s, a);
   return (int)hipGetLastError();
+}
+// sequences that the scan has places for
+int places(const PrefillArgs& a) {
+  const int most = (int)std::min<int64_t>(chunked_most(a.T, a.N, a.chunk_from), 64);
+  return a.N / 64 * most + std::min(a.N % 64, most);
 }
 template <class Act, class St, bool SPLIT, int WAVES, bool ROLES>
 int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
@@ -1128,7 +1181,7 @@ int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
   const auto kernel = chunk_scan_kernel<Act, St, SPLIT, WAVES, ROLES>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(kernel, dim3(a.HV * (a.V / (ROLES ? 16 : 16 * WAVES)), a.N), dim3(64 * WAVES), lds, s, a);
+  hipLaunchKernelGGL(kernel, dim3(a.HV * (a.V / (ROLES ? 16 : 16 * WAVES)), places(a)), dim3(64 * WAVES), lds, s, a);
   return (int)hipGetLastError();
 }
 // A workgroup's LDS leaves room for one on a compute unit, so the scan's time is
@@ -1143,7 +1196,7 @@ int launch_scan_as(const PrefillArgs& a, hipStream_t s) {
 // 67, 65 and 71; 16: 137, 164 and 185, with 8 waves 105.
 template <class Act, class St, bool SPLIT>
 int launch_scan(const PrefillArgs& a, hipStream_t s) {
-  const int64_t rows = (int64_t)a.N * a.HV * a.V, cus = device_cus();
+  const int64_t rows = (int64_t)places(a) * a.HV * a.V, cus = device_cus();
   const auto cost = [&](int columns, int chunk) {
     return a.V % columns ? INT64_MAX : (rows / columns + cus - 1) / cus * chunk;
   };
@@ -1164,36 +1217,32 @@ int launch_recurrent(const PrefillArgs& a, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+template <class Act, class St, bool GATE_F32>
+int launch_forms(const PrefillArgs& a, hipStream_t s) {
+  constexpr bool SPLIT = !(std::is_same<Act, ActBF16>::value && std::is_same<St, ActBF16>::value);
+  int rc = a.chunk_from ? launch_recurrent<Act, St, GATE_F32>(a, s) : 0;
+  if (rc || a.chunk_from == INT32_MAX) return rc;
+  rc = launch_prep<Act, GATE_F32, SPLIT>(a, s);
+  return rc ? rc : launch_scan<Act, St, SPLIT>(a, s);
+}
 template <class Act, bool GATE_F32>
 int launch_state(const PrefillArgs& a, int state_dt, hipStream_t s) {
-  constexpr int ACT = std::is_same<Act, ActBF16>::value ? DT_BF16 : std::is_same<Act, ActF16>::value ? DT_F16 : DT_F32;
-  if (chunked_form(a.T, a.N, needs_split(ACT, state_dt))) {
-    if constexpr (std::is_same<Act, ActBF16>::value) {
-      if (state_dt == DT_BF16) {
-        const int rc = launch_prep<Act, GATE_F32, false>(a, s);
-        return rc ? rc : launch_scan<Act, ActBF16, false>(a, s);
-      }
-    }
-    const int rc = launch_prep<Act, GATE_F32, true>(a, s);
-    if (rc) return rc;
-    if (state_dt == DT_F16) return launch_scan<Act, ActF16, true>(a, s);
-    if (state_dt == DT_F32) return launch_scan<Act, ActF32, true>(a, s);
-    if constexpr (!std::is_same<Act, ActBF16>::value) return launch_scan<Act, ActBF16, true>(a, s);
-  }
-  if (state_dt == DT_BF16) return launch_recurrent<Act, ActBF16, GATE_F32>(a, s);
-  if (state_dt == DT_F16) return launch_recurrent<Act, ActF16, GATE_F32>(a, s);
-  return launch_recurrent<Act, ActF32, GATE_F32>(a, s);
+  if (state_dt == DT_BF16) return launch_forms<Act, ActBF16, GATE_F32>(a, s);
+  if (state_dt == DT_F16) return launch_forms<Act, ActF16, GATE_F32>(a, s);
+  return launch_forms<Act, ActF32, GATE_F32>(a, s);
 }
 
 }  // namespace
 
 int64_t prefill_work_bytes(int64_t T, int64_t N, int32_t H, int32_t HV, int act_dt, int state_dt) {
   const bool split = needs_split(act_dt, state_dt);
-  if (!chunked_form(T, N, split)) return 0;
-  return (T / C + N) * (H * unit_bytes(split) + HV * head_bytes(split));
+  const int32_t from = chunk_start(T, N, split);
+  return from == INT32_MAX ? 0 : chunk_slots(T, N, from) * (H * unit_bytes(split) + HV * head_bytes(split));
 }
 
-int launch_prefill(const PrefillArgs& a, int state_dt, int act_dt, bool gate_f32, void* stream) {
+int launch_prefill(const PrefillArgs& args, int state_dt, int act_dt, bool gate_f32, void* stream) {
+  PrefillArgs a = args;
+  a.chunk_from = chunk_start(a.T, a.N, needs_split(act_dt, state_dt));
   hipStream_t s = (hipStream_t)stream;
   if (act_dt == DT_F32) return launch_state<ActF32, true>(a, state_dt, s);
   if (act_dt == DT_BF16) return gate_f32 ? launch_state<ActBF16, true>(a, state_dt, s) : launch_state<ActBF16, false>(a, state_dt, s);

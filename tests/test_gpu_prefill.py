@@ -338,3 +338,36 @@ def test_large_keys_and_queries(device, lengths, act, magnitude):
     x["mixed"][::2, :512] *= magnitude
     x["mixed"][1::4, :256] *= magnitude  # (queries alone)
     check(x)
+
+
+# fewer than 16 tokens a sequence on average (32 with wider results), some of a chunk and more among them
+SHORT_AND_LONG = {"one": [150] + [1] * 20, "edges": [1, 63, 64, 0, 65] + [2] * 30, "last": [1] * 40 + [0, 333],
+                  "groups": [1] * 60 + [70, 130, 1, 64, 64, 128] + [0, 3] * 40 + [65] + [1] * 9, "none long": [9] * 20,
+                  "all in one": [0] * 70 + [200] + [0] * 5}
+
+
+@pytest.mark.parametrize("name", SHORT_AND_LONG)
+@pytest.mark.parametrize("act,state", [(BF16, BF16), (F16, F32), (F32, F32), (BF16, F32)])
+def test_long_sequences_among_short(device, name, act, state):
+    """Short sequences token by token and long ones in chunks, in one call:
+    nothing past the workspace that was asked for is written, nothing that it held is
+    read."""
+    lengths = SHORT_AND_LONG[name]
+    assert 128 <= sum(lengths) < 16 * len(lengths)
+    x = make(lengths, device, seed=42, act=act, state=state, started=[n % 3 != 1 for n in range(len(lengths))])
+    x["state"][x["slots"][1::3].long()] = float("nan")  # (their sequences start from nothing)
+    size = gdnr_lib.prefill_workspace(sum(lengths), len(lengths), 2, 4, 128, act, state)
+    assert size > 0
+    workspace = torch.full((size + 4096,), 0xFF, dtype=torch.uint8, device=device)
+    check(x, workspace=workspace[:size])
+    assert (workspace[size:] == 0xFF).all()
+
+
+def test_long_among_short_is_the_long_one_alone(device):
+    """What a long sequence gets does not depend on the short ones beside it."""
+    x = make([1] * 30 + [200], device, seed=43, heads=8, value_heads=16)
+    y = dict(x, mixed=x["mixed"][30:], a=x["a"][30:], b=x["b"][30:], slots=x["slots"][30:],
+             cu=torch.tensor([0, 200], dtype=torch.int32, device=device), state=x["state"].clone())
+    whole, alone = run(x), run(y)
+    slot = int(x["slots"][30])
+    assert torch.equal(whole[30:], alone) and torch.equal(x["state"][slot], y["state"][slot])

@@ -274,3 +274,14 @@ def test_a_prompt_in_one_piece_takes_none_beside_a_decode():
     assert gdnr_lib.paged_attention_workspace(8192, 1, 32, 8, 128, 131072) == 0
     size = gdnr_lib.paged_attention_workspace(8193, 2, 32, 8, 128, 131072)
     assert 0 < size <= 2 * 8 * 256 * 16 * 4 * (128 + 2)
+
+
+@pytest.mark.parametrize("state", [torch.bfloat16, torch.float32])
+def test_a_long_prompt_among_single_tokens_is_walked_in_chunks(state):
+    """900 tokens beside 63 sequences of one: a workspace for the prompt's
+    chunks, which its tokens alone would take too, and little more; none where no
+    sequence can be long."""
+    size = lambda tokens, sequences: gdnr_lib.prefill_workspace(tokens, sequences, 16, 32, 128, torch.bfloat16, state)  # noqa: E731
+    assert size(900, 1) <= size(963, 64) <= 2 * size(900, 1)
+    assert size(2000, 1000) <= 2 * size(2000, 1)
+    assert size(8 * 4, 8) == size(64, 64) == 0
