@@ -200,8 +200,9 @@ __global__ __launch_bounds__(256) void recurrent_kernel(const PrefillArgs a) {
 // Numbers: the products run on f16 operands with f32 sums. Unit keys and
 // queries, A and T (|T| <= 1: products of contractions) are safe in f16; V,
 // S0, R and U get a power of two per V-row and chunk, from the largest of the
-// row's v and state, that puts their bound at 2^15 (V-rows do not mix, so each
-// keeps its own precision whatever its neighbours hold). An f16 operand costs
+// row's v and state, that keeps them in range (V-rows do not mix, so each
+// keeps its own precision whatever its neighbours hold; a chunk whose tokens
+// differ too much for one such factor is walked token by token). An f16 operand costs
 // 2^-12 of itself, an eighth of what storing bf16 does: bf16 outputs and states
 // are bound by their own rounding. Where a result keeps more than bf16 (f16
 // or f32 activations or state), SPLIT carries every operand as a sum of two
@@ -266,7 +267,7 @@ __device__ __forceinline__ f32x4_t product(const Operand<SPLIT>& a, const Operan
 // Workspace: per chunk slot and key head the unit keys and queries [C][K] f16
 // (SPLIT: high, then low), a row's pieces as unit_at places them; per slot and
 // value head the tokens' {beta}[C], {-beta e^G}[C], {e^(G_C - G)}[C], {e^G}[C],
-// first bad token (an int), padded to 2 KiB, then the operand tiles of T - I and
+// first bad token (an int) in 64 words, {e^g}[C], padded to 2 KiB, then the operand tiles of T - I and
 // of A (64 lanes x 16 bytes each; SPLIT: high, then low). The chunks
 // of a sequence take slots one after the other.
 constexpr int kScalars = 2048;
@@ -501,6 +502,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 :
       sc[2 * C + t] = exp2_diff<SPLIT>(end, G);
       sc[3 * C + t] = grow;
       if (t == 0) ((int*)sc)[4 * C] = first;
+      sc[5 * C + t] = expf(g);
     }
     __syncthreads();
 #pragma nounroll
@@ -616,6 +618,14 @@ __device__ __forceinline__ float column_max(float x) {
   const uint32_t h = __float_as_uint(__builtin_elementwise_maximum(__uint_as_float(half[0]), __uint_as_float(half[1])));
   const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
   return __builtin_elementwise_maximum(__uint_as_float(row[0]), __uint_as_float(row[1]));
+}
+
+// (code that is left out of the way of what runs for every chunk)
+__device__ __forceinline__ bool rare(bool x) { return __builtin_expect(x, false); }
+// whether each of the 16 columns has a lane in the mask
+__device__ __forceinline__ bool all_columns(uint64_t lanes) {
+  lanes |= lanes >> 32;
+  return ((lanes | lanes >> 16) & 0xFFFF) == 0xFFFF;
 }
 
 // Of a 16-row tile as a product leaves it (rows 4 grp + j, column lane & 15),
@@ -844,6 +854,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   };
   bool any_bad = false;
   int first = C;  // first token of the chunk whose results are NaN in this V-row
+  bool by_token = false;  // the chunk's outputs are written already
+  const float not_first = grp == 0 ? 0.f : __builtin_inff();
 
   // what is handed over: operands of S (0 .. 3) and U (4, 5), then scale and first
   // bad token; SPLIT: the operands' low halves after that
@@ -852,6 +864,68 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
   auto hand_over = [&](int c, int i, const Operand<SPLIT>& o) {
     *place(c, i) = o.hi;
     if constexpr (SPLIT) *place(c, kLow + i) = o.lo;
+  };
+
+  // A chunk token by token in f32, from its keys in LDS and its queries where the
+  // preparation left them: the state and the outputs. (53 us a chunk, 106 SPLIT: for
+  // rows that hold values of very different magnitude.)
+  auto walk = [&](int c, const uint8_t* b, const float* scal) {
+    const uint8_t* queries = unit + c * unit_step + plane_bytes(SPLIT);
+    uint8_t* orow = op + c * C * o_row + (int64_t)v0 * ES;
+    auto four = [](const uint8_t* p, float* x) {
+      const uint2 w = *(const uint2*)p;
+      const float2 lo = unpack_f16(w.x), hi = unpack_f16(w.y);
+      x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+      if constexpr (SPLIT) {
+        const uint2 u = *(const uint2*)(p + plane_bytes(false));
+        const float2 l = unpack_f16(u.x), h = unpack_f16(u.y);
+        x[0] = kDown * (x[0] + l.x), x[1] = kDown * (x[1] + l.y), x[2] = kDown * (x[2] + h.x), x[3] = kDown * (x[3] + h.y);
+      }
+    };
+    auto total_of = [](float x) {  // over the lanes of a column
+      x += __shfl_xor(x, 16);
+      return x + __shfl_xor(x, 32);
+    };
+#pragma unroll
+    for (int kt = 0; kt < 8; ++kt) S[kt] *= inv;
+    sc = 1.f, inv = 1.f;
+    const int count = min(C, len - c * C);
+#pragma nounroll
+    for (int t = 0; t < count; ++t) {
+      float x;
+      if constexpr (ROLES) x = Act::ld(lds + L::VALUES_AT + (c & 1) * L::VALUES + 16 * ES * t, col);
+      else x = Act::ld(vp + (c * C + t) * v_row, v0);
+      if (!finite(x)) x = 0.f;
+      const float beta = scal[t], gamma = scal[5 * C + t];
+      // (operands are read where they are used, four tiles at a time: kept over the
+      // token they would cost the other path registers)
+      float x4[4], sk = 0.f, o = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < 8; ++kt) {
+        if (kt % 4 == 0) GDNR_COMPILER_FENCE();
+        four(b + unit_at(t, 4 * kt + grp), x4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) S[kt][j] *= gamma, sk = fmaf(S[kt][j], x4[j], sk);
+      }
+      const float u = beta * (x - total_of(sk));
+#pragma unroll
+      for (int kt = 0; kt < 8; ++kt) {
+        if (kt % 4 == 0) GDNR_COMPILER_FENCE();
+        four(b + unit_at(t, 4 * kt + grp), x4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) S[kt][j] = fmaf(u, x4[j], S[kt][j]);
+        four(queries + unit_at(t, 4 * kt + grp), x4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o = fmaf(S[kt][j], x4[j], o);
+      }
+      GDNR_COMPILER_FENCE();
+      o = a.out_scale * total_of(o);
+      if (grp == 0) Act::st(orow + t * o_row, 0, t >= first ? __builtin_nanf("") : o);
+    }
+    if (any_bad && first < C) {
+#pragma unroll
+      for (int kt = 0; kt < 8; ++kt) S[kt] = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+    }
   };
 
   // the chain: chunk c's R and U from S, then S after it
@@ -895,7 +969,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = Act::from_bits(vn[i]);
     }
-    if ((c + 1) * C > len) {
+    if (rare((c + 1) * C > len)) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (c * C + 16 * (i >> 2) + 4 * grp + (i & 3) >= len) v[i >> 2][i & 3] = 0.f;
@@ -908,21 +982,39 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     for (int s = 0; s < AHEAD; ++s) read_rows(b, s);
     GDNR_COMPILER_FENCE();
 
-    // V-rows with a value that is not finite: zeros here, NaN from its token on
-    float bound;  // |R| and |U| are at most 64 (|v| + 12 |S|)
+    // |S k| is at most |S| as a vector, and a token adds at most its v to that, at a
+    // right angle or less: |R| and |U| are at most 10 times the bound. A row's f16
+    // operands are off by some 2^-33 of it. Where a token that is much smaller may need
+    // what that rounds off, the chunk is walked token by token: a later token's v, or a
+    // state that has decayed meanwhile, must not cost it its bits. That needs four tokens
+    // that are all that small, or one of the chunk's first (SPLIT: in four rows).
+    constexpr float kSmall = SPLIT ? 0x1p-9f : 0x1p-18f;
+    float bound, state_part, least;
+    auto of_four_rows = [](float x) {
+      x = __builtin_fabsf(x);
+      x = fmaxf(x, dpp_f<kDppXor1>(x));
+      return fmaxf(x, dpp_f<kDppXor2>(x));
+    };
     auto largest = [&]() {
-      float x = 0.f, x2 = 0.f, y = 0.f;
+      float x = 0.f, x2 = 0.f, y[4];
 #pragma unroll
       for (int kt = 0; kt < 8; ++kt) x = max3_abs(x, S[kt][0], S[kt][1]), x2 = max3_abs(x2, S[kt][2], S[kt][3]);
-      x = __builtin_elementwise_maximum(x, x2);
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) y = max3_abs(y, v[i >> 2][i & 3], v[i >> 2][(i & 3) + 1]);
-      bound = column_max(max3_abs(12.f * inv * x, y, 0.f));
+      for (int tt = 0; tt < 4; ++tt) y[tt] = max3_abs(max3_abs(0.f, v[tt][0], v[tt][1]), v[tt][2], v[tt][3]);
+      if constexpr (SPLIT) least = fminf(fminf(of_four_rows(v[0][0]), of_four_rows(v[0][1])), of_four_rows(v[0][2]));
+      else least = fminf(fminf(__builtin_fabsf(v[0][0]), __builtin_fabsf(v[0][1])), __builtin_fabsf(v[0][2]));
+      least = fminf(fmaxf(least, not_first), y[0]);
+      least = fminf(fminf(fminf(least, 0x1p127f), y[1]), fminf(y[2], y[3]));
+      state_part = 12.f * inv * __builtin_elementwise_maximum(x, x2);
+      bound = column_max(max3_abs(max3_abs(state_part, y[0], y[1]), y[2], y[3]));
     };
     largest();
     first = C;
-    any_bad = bad_token < C || __any(!finite(bound));
-    if (any_bad) {
+    any_bad = by_token = false;
+    if (rare(bad_token < C || __ballot(!(least >= kSmall * bound)) != 0)) {
+      // V-rows with a value that is not finite (the bound then neither): zeros here, NaN
+      // from its token on
+      any_bad = bad_token < C || __ballot(!finite(bound)) != 0;
       float at = C;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -936,13 +1028,30 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
           if (!finite(S[kt][j])) S[kt][j] = 0.f, at = 0.f;
       first = min(C - (int)column_max(C - at), bad_token);
       largest();
+      // a row is safe where what it starts with, decayed by the whole chunk, is not
+      // small; or where no token's v of it and its three neighbours is
+      const float start = fmaxf(state_part, grp == 0 ? __builtin_fabsf(v[0][0]) : 0.f);
+      const uint64_t safe = __ballot(total * start >= kSmall * bound);
+      least = __builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = of_four_rows(v[i >> 2][i & 3]);
+        if (c * C + 16 * (i >> 2) + 4 * grp + (i & 3) < len) least = fminf(least, x);
+      }
+      least = -column_max(-least);
+      by_token = !all_columns(safe | __ballot(least >= kSmall * bound));
+      if (by_token) {
+        walk(c, b, scal);
+        if constexpr (ROLES) *place(c, 6) = u32x4_t{0, 0, 0, 1};
+        return;
+      }
     }
-    // Each row's power of two puts 64 times its bound between 2^9 and 2^15. It
-    // stays what it was while it does: then nothing is rescaled.
+    // Each row's power of two puts its bound between 2^8 and 2^12. It stays what
+    // it was while it does: then nothing is rescaled.
     float ratio = 1.f;
     const float scaled = bound * sc;
-    if (!(scaled < 0x1p8f && scaled >= 0x1p2f)) {
-      const uint32_t ex = min(max((__float_as_uint(bound) >> 23) + 7, 21u), 254u);
+    if (!(scaled < 0x1p12f && scaled >= 0x1p8f)) {
+      const uint32_t ex = min(max((__float_as_uint(bound) >> 23) + 3, 21u), 257u);
       const float s_new = __uint_as_float((268u - ex) << 23);
       ratio = fminf(s_new * inv, 0x1p126f);
       sc = s_new, inv = __uint_as_float((ex - 14u) << 23);
@@ -956,7 +1065,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       bs[s] = operand<SPLIT>(S[2 * s], S[2 * s + 1]);
       if constexpr (ROLES) hand_over(c, s, bs[s]);
     }
-    if constexpr (ROLES) *place(c, 6) = u32x4_t{__float_as_uint(inv), (uint32_t)first, any_bad, 0};
+    if constexpr (ROLES) *place(c, 6) = u32x4_t{__float_as_uint(inv), (uint32_t)first, any_bad, by_token};
 
     f32x4_t u[4];
     by_state(b, u);  // K S0^T
@@ -1018,7 +1127,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
       for (int kt = 0; kt < 8; ++kt) S[kt] *= kDown;
     }
-    if (any_bad && first < C) {
+    if (rare(any_bad) && first < C) {
 #pragma unroll
       for (int kt = 0; kt < 8; ++kt) S[kt] = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
     }
@@ -1047,7 +1156,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const float scale = kDown * a.out_scale * inv;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) o[tt] *= scale;
-    if (any_bad) {
+    if (rare(any_bad)) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (16 * (i >> 2) + 4 * grp + (i & 3) >= first) o[i >> 2][i & 3] = __builtin_nanf("");
@@ -1064,7 +1173,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     uint8_t* orow = op + c * C * o_row + o_lane;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
-      store_turned<Act>(orow + 16 * tt * o_row, o[tt], lane, c * C + 16 * tt + 4 * grp + (lane & 3) < len);
+      store_turned<Act>(orow + 16 * tt * o_row, o[tt], lane, !by_token && c * C + 16 * tt + 4 * grp + (lane & 3) < len);
   };
 
   if (chain) {
@@ -1098,6 +1207,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
           }
           const u32x4_t x = *place(c - 1, 6);
           inv = __uint_as_float(x[0]), first = (int)x[1], any_bad = __builtin_amdgcn_readfirstlane(x[2]) != 0;
+          by_token = __builtin_amdgcn_readfirstlane(x[3]) != 0;
         }
         if (L::BUFS == 1 && c == 0 && chunks) fetch_queries(0);
       }

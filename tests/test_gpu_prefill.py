@@ -371,3 +371,31 @@ def test_long_among_short_is_the_long_one_alone(device):
     whole, alone = run(x), run(y)
     slot = int(x["slots"][30])
     assert torch.equal(whole[30:], alone) and torch.equal(x["state"][slot], y["state"][slot])
+
+
+@pytest.mark.parametrize("act,state", [(BF16, BF16), (F32, F32), (BF16, F32)])
+@pytest.mark.parametrize("sequences", [1, 9, 40])  # (roles; several waves a workgroup)
+@pytest.mark.parametrize("token", [1, 4, 50, 63])
+@pytest.mark.parametrize("magnitude", [1e2, 1e4, 1e6, 1e8, 1e12, 1e30])
+def test_a_large_value_costs_earlier_tokens_nothing(device, act, state, sequences, token, magnitude):
+    """One V-row's v far above everything at one token: the outputs before it, of
+    that row alone, are as good as without it, and so is what follows."""
+    x = make([70] * sequences, device, seed=44, heads=1, value_heads=2, act=act, state=state)
+    at = torch.arange(sequences, device=device) * 70 + token
+    x["mixed"][at, 256 + 5] = magnitude
+    want, _ = expected(x)
+    out = np64(check(x)).reshape(sequences, 70, 2, 128)[:, :token, 0, 5]
+    assert rel_l2(out, want.reshape(sequences, 70, 2, 128)[:, :token, 0, 5]) <= TOL[act]
+
+
+@pytest.mark.parametrize("act,state", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("magnitude", [1e4, 1e8, 1e15])
+def test_a_state_forgotten_costs_later_tokens_nothing(device, act, state, magnitude):
+    """A large state that the first tokens' decay forgets: what is left is as
+    precise as if it had never been there."""
+    x = make([100], device, seed=45, act=act, state=state)
+    x["state"] *= magnitude
+    x["a"][3:20] += 20.0  # (log decays of some -17 to -50 each)
+    want, _ = expected(x)
+    out = np64(check(x))
+    assert rel_l2(out[20:], want[20:]) <= TOL[act]
