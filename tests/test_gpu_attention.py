@@ -381,3 +381,17 @@ def test_append_large_rows(device, dim, rotary, interleaved, magnitude):
     x["k"][1::3, 0] *= magnitude
     check_append(x, interleaved=interleaved)
     check_append(x, interleaved=interleaved, eps=1e10)
+
+
+@pytest.mark.parametrize("new,context,heads,kv_heads,dim,turns", [
+    (180, 190, 256, 64, 64, 1.5), (250, 256, 256, 64, 64, 2.0), (75, 200, 1024, 128, 64, 2.5), (250, 700, 256, 64, 128, 2.0),
+    (33, 250, 1024, 128, 256, 2.5)])
+def test_order_of_the_tiles_past_one_to_a_compute_unit(device, new, context, heads, kv_heads, dim, turns):
+    """One sequence in one piece, with ``turns`` times as many tiles as one to
+    each compute unit: the second ones are taken from the other end, the rest in order."""
+    rows, group = 64 if dim == 256 else 128, heads // kv_heads
+    tiles, places = -(-new // (rows // group)), torch.cuda.get_device_properties(device).multi_processor_count // kv_heads
+    if torch.cuda.get_device_properties(device).multi_processor_count == 256:
+        assert tiles == turns * places
+    assert gdnr_lib.paged_attention_workspace(new, 1, heads, kv_heads, dim, context) == 0  # one piece
+    check_attention(make_attention([new], [context], device, heads=heads, kv_heads=kv_heads, dim=dim, seed=new), max_context=context)
