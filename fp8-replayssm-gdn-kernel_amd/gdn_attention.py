@@ -37,10 +37,10 @@ def rope_table(positions: int, rotary_dim: int, base: float = 10000.0, device="c
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even")
     if inv_freq is None:
-        inv_freq = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+        inv_freq = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device="cpu") / rotary_dim)
     if tuple(inv_freq.shape) != (rotary_dim // 2,):
         raise ValueError("inv_freq must be [rotary_dim / 2]")
-    angle = torch.arange(positions, dtype=torch.float64)[:, None] * inv_freq.double().cpu()
+    angle = torch.arange(positions, dtype=torch.float64, device="cpu")[:, None] * inv_freq.double().cpu()
     return (torch.cat([angle.cos(), angle.sin()], dim=-1) * scale).float().to(device)
 
 

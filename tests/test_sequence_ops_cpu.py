@@ -285,3 +285,12 @@ def test_a_long_prompt_among_single_tokens_is_walked_in_chunks(state):
     assert size(900, 1) <= size(963, 64) <= 2 * size(900, 1)
     assert size(2000, 1000) <= 2 * size(2000, 1)
     assert size(8 * 4, 8) == size(64, 64) == 0
+
+
+def test_rope_table_under_any_default_device():
+    """The angles are formed on the host whatever torch's default device is."""
+    want = ga.rope_table(20, 16, device="cpu")
+    freq = 10000.0 ** (-torch.arange(0, 16, 2, dtype=torch.float64) / 16)
+    with torch.device("meta"):
+        got, given = ga.rope_table(20, 16, device="cpu"), ga.rope_table(20, 16, device="cpu", inv_freq=freq)
+    assert torch.equal(got, want) and torch.equal(given, want)
