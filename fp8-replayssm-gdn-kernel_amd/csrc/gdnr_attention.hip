@@ -72,17 +72,17 @@ __device__ __forceinline__ uint2 transposed4(const uint8_t* p) {
 // A weight is 2^(score - reference). f16 has all its bits down to 2^-14 alone,
 // and a long tail of small weights under one large key is what the output consists of
 // where that key's value is 0: there the reference lies kHead below the
-// maximum that it was taken from, so that a weight that is 2^-27 of the largest keeps
-// all its bits and one of 2^-38 still counts. kLag: how far tile_kernel's scores
+// maximum that it was taken from, so that a weight that is 2^-25 of the largest keeps
+// all its bits and one of 2^-36 still counts. kLag: how far tile_kernel's scores
 // may pass that maximum before the reference follows; 2^(kHead + kLag + 1/2) fits
 // the type. (With a lag of 8 and no head, thousands of keys 18 below one whose value
 // is 0 gave outputs off by 0.7 to 6.7%; f16 rounds to 0.02%.) bf16 has f32's exponents.
 template <class Act>
 constexpr bool is_f16() { return !std::is_same<Act, ActBF16>::value; }
 template <class Act>
-constexpr float kHead = is_f16<Act>() ? 13.f : 0.f;
+constexpr float kHead = is_f16<Act>() ? 11.f : 0.f;
 template <class Act>
-constexpr float kLag = is_f16<Act>() ? 2.f : 8.f;
+constexpr float kLag = is_f16<Act>() ? 4.f : 8.f;
 // whether a maximum has passed the reference's own by more than lag (a
 // difference: exact where they are large)
 template <class Act>

@@ -399,3 +399,31 @@ def test_a_state_forgotten_costs_later_tokens_nothing(device, act, state, magnit
     want, _ = expected(x)
     out = np64(check(x))
     assert rel_l2(out[20:], want[20:]) <= TOL[act]
+
+
+@pytest.mark.parametrize("act,state", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("sequences", [1, 40])
+def test_large_and_nonfinite_values_in_one_chunk(device, act, state, sequences):
+    """A V-row that is NaN from its token on, and a key head whose key is, in
+    chunks that are walked token by token for another row's large value."""
+    x = make([90] * sequences, device, seed=46, heads=2, value_heads=4, act=act, state=state)
+    want, want_state = expected(x)
+    rows = torch.arange(sequences, device=device) * 90
+    x["mixed"][rows + 40, 512 + 5] = 1e12  # value head 0
+    x["mixed"][rows + 50, 512 + 9] = float("nan")
+    x["mixed"][rows + 60, 256 + 128 + 3] = float("inf")  # the key of value heads 2 and 3
+    x["mixed"][rows + 20, 512 + 2 * 128 + 7] = 1e12  # value head 2
+    large, _ = expected(x)
+    out = np64(run(x)).reshape(sequences, 90, 4, 128)
+    want, large = want.reshape(out.shape), large.reshape(out.shape)
+    assert np.isnan(out[:, 50:, 0, 9]).all() and np.isnan(out[:, 60:, 2:]).all()
+    others = [r for r in range(128) if r not in (5, 9)]
+    assert rel_l2(out[:, :, 0, others], want[:, :, 0, others]) <= TOL[act]
+    assert rel_l2(out[:, :50, 0, 9], want[:, :50, 0, 9]) <= TOL[act]
+    assert rel_l2(out[:, :, 1], want[:, :, 1]) <= TOL[act]
+    assert rel_l2(out[:, :40, 0, 5], want[:, :40, 0, 5]) <= TOL[act]
+    assert rel_l2(out[:, 40:, 0, 5], large[:, 40:, 0, 5]) <= TOL[act]
+    assert rel_l2(out[:, :60, 3], want[:, :60, 3]) <= TOL[act]
+    assert rel_l2(out[:, :20, 2, 7], want[:, :20, 2, 7]) <= TOL[act]
+    states = np64(x["state"])[x["slots"].cpu().numpy()]
+    assert np.isnan(states[:, 0, 9]).all() and np.isnan(states[:, 2:]).all() and np.isfinite(states[:, 0, others]).all()
