@@ -1553,7 +1553,7 @@ int gdnr_paged_attention(const gdnr_tensor* q, const gdnr_tensor* k_cache, const
   r.q = q->data, r.q_t = q->strides[0], r.q_h = q->strides[1];
   r.k_cache = k_cache->data, r.kc_p = k_cache->strides[0], r.kc_t = k_cache->strides[1], r.kc_h = k_cache->strides[2];
   r.v_cache = v_cache->data, r.vc_p = v_cache->strides[0], r.vc_t = v_cache->strides[1], r.vc_h = v_cache->strides[2];
-  r.table = (const int32_t*)block_table->data, r.tb_n = block_table->strides[0], r.table_width = (int32_t)block_table->shape[1];
+  r.table = (const int32_t*)block_table->data, r.tb_n = block_table->strides[0];
   r.cu = (const int32_t*)cu_seqlens->data, r.cu_s = cu_seqlens->strides[0];
   r.context = (const int32_t*)context_lens->data, r.cx_s = context_lens->strides[0];
   r.out = out->data, r.o_t = out->strides[0], r.o_h = out->strides[1];

@@ -210,7 +210,7 @@ struct AttentionArgs {
   const void* q; int64_t q_t, q_h;
   const void* k_cache; int64_t kc_p, kc_t, kc_h;
   const void* v_cache; int64_t vc_p, vc_t, vc_h;
-  const int32_t* table; int64_t tb_n; int32_t table_width;
+  const int32_t* table; int64_t tb_n;
   const int32_t* cu; int64_t cu_s;
   const int32_t* context; int64_t cx_s;
   void* out; int64_t o_t, o_h;
