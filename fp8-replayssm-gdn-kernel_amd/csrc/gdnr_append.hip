@@ -11,9 +11,9 @@
 // instruction moves 512 / D heads; a wave walks the heads of one token and
 // keeps its table row and the weights in registers. The pair's other element
 // sits rotary / 16 lanes away (a lane exchange of the raw bits) or in the same
-// lane (interleaved). 8192 tokens of 32 + 2 x 8 heads of 128 take 47.9 us (4.3
+// lane (interleaved). 8192 tokens of 32 + 2 x 8 heads of 128 take 47.4 us (4.3
 // TB/s, 0.87 of a copy's rate), 14001 tokens of heads of 64, interleaved, 69.9 (as a
-// copy); one token takes 3.8 us, its chain of loads.
+// copy); one token takes 3.4 us, its chain of loads.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

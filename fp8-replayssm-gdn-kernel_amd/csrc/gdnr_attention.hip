@@ -21,7 +21,7 @@
 // tile_kernel: the others. Bound by the matrix products and the exponentials:
 // 128 rows a workgroup (64 at D = 256), 32 (16) a wave, all on the same keys.
 // 2048 tokens over 8192 keys, 32 heads of 128: 248 us, 969 TFLOP/s (a square
-// product of 8192 in the library: 1130).
+// product of 8192 in the library: 1130); 32 of 64 159 us, 757; 16 of 256 320, 752.
 // A context is cut into pieces where the rows alone do not fill the card, and
 // join_kernel adds the pieces in their order.
 #include <hip/hip_runtime.h>

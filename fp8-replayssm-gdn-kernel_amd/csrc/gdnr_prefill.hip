@@ -81,7 +81,7 @@ __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)
 // value head, a lane 8 columns of 4 of them, in registers from the first token
 // to the last. Rows of S are independent, so nothing is shared between waves.
 // One read and one write of the state carry a call of a few tokens (8 sequences
-// of 4 tokens, HV=32, V=128, bf16: 9.0 us, of which the 15.5 MB of states and
+// of 4 tokens, HV=32, V=128, bf16: 9.1 us, of which the 15.5 MB of states and
 // rows take 3.1 at a copy's rate; launch, the reads' latency and 240 instructions
 // a token and wave the rest, one after the other since all waves start together).
 // A long sequence is bound by the chain of a token's row sums (S k must be known
@@ -358,8 +358,8 @@ __device__ __forceinline__ double prefix_sum(double x, double& total) {
 // One chunk of one key head: 4 waves. The Gram products are formed transposed
 // (rows i on a lane's registers, columns t on lanes), which is the order that
 // the scan's operands take them in. Bound by its bytes: 8192 tokens of 16 key and
-// 32 value heads read 68 MB and write 126 MB of operands in 51 us (3.8 TB/s, three
-// quarters of a copy's rate); one workgroup alone takes 11.9 us, which four of
+// 32 value heads read 84 MB and write 123 MB (counters) in 52 us (4.0 TB/s, four fifths
+// of a copy's rate); one workgroup alone takes 11.9 us, which four of
 // them a compute unit cover.
 template <class Act, bool GATE_F32, bool SPLIT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(SPLIT ? 2 : 4, SPLIT ? 2 : 4))) void chunk_prep_kernel(const PrefillArgs a) {
@@ -722,8 +722,8 @@ struct ScanLds {
 // either reads (48 copies a chunk, whose issue alone costs a wave 850 cycles).
 // Otherwise WAVES waves do all of it for 16 V-rows each on shared operands.
 //
-// Bound by the chain: 128 chunks of one sequence, HV=32, V=128, bf16 take 165 us,
-// 1.3 a chunk (2500 cycles of the chain's wave: 230 vector instructions of 4
+// Bound by the chain: 128 chunks of one sequence, HV=32, V=128, bf16 take 173 us,
+// 1.35 a chunk (2600 cycles of the chain's wave: 240 vector instructions of 4
 // cycles and 38 products of 16 one after the other, and the latencies between
 // them; the outputs' wave has 1600 to do). With 8 waves a workgroup two waves a
 // SIMD hide half of each other's latency: 3.7 us a chunk of 128 V-rows.

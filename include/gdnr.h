@@ -384,7 +384,8 @@ int gdnr_prefill(const gdnr_tensor* mixed_qkv, const gdnr_tensor* a, const gdnr_
                  const gdnr_tensor* has_initial_state, const gdnr_tensor* out,
                  const gdnr_tensor* workspace, float scale, void* stream);
 
-/* Bytes of workspace of a gdnr_prefill call (-1: invalid arguments). Host-only. */
+/* Bytes of workspace of a gdnr_prefill call (-1: invalid arguments). Host-only.
+ * value_dim does not change it at present. */
 int64_t gdnr_prefill_workspace(int64_t tokens, int64_t sequences, int32_t heads, int32_t value_heads,
                                int32_t value_dim, int32_t act_dtype, int32_t state_dtype);
 
