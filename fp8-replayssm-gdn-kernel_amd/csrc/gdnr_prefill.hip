@@ -267,9 +267,9 @@ __device__ __forceinline__ f32x4_t product(const Operand<SPLIT>& a, const Operan
 // Workspace: per chunk slot and key head the unit keys and queries [C][K] f16
 // (SPLIT: high, then low), a row's pieces as unit_at places them; per slot and
 // value head the tokens' {beta}[C], {-beta e^G}[C], {e^(G_C - G)}[C], {e^G}[C],
-// first bad token (an int) in 64 words, {e^g}[C], padded to 2 KiB, then the operand tiles of T - I and
-// of A (64 lanes x 16 bytes each; SPLIT: high, then low). The chunks
-// of a sequence take slots one after the other.
+// first bad token (an int) in 64 words, {e^g}[C], padded to 2 KiB, then the operand
+// tiles of T - I and of A (64 lanes x 16 bytes each; SPLIT: high, then low). The
+// chunks of a sequence take slots one after the other.
 constexpr int kScalars = 2048;
 __host__ __device__ constexpr int64_t plane_bytes(bool split) { return C * K * 2 * (split ? 2 : 1); }  // keys, or queries
 __host__ __device__ constexpr int64_t unit_bytes(bool split) { return 2 * plane_bytes(split); }
@@ -665,9 +665,10 @@ __device__ __forceinline__ void dma_part(const uint8_t* src, uint32_t lds_addr, 
 }
 
 // The sequence at a place of the launch's order (-1: none) and its first slot: of each
-// 64 sequences those of most chunks first. Workgroups start in order as others end, so that the last to start are
-// then short ones (24 sequences of up to 1096 tokens: the scan 186 us as given,
-// 168 so). The place is looked for bit by bit of the chunk counts.
+// 64 sequences those of most chunks first. Workgroups start in order as others end,
+// so that the last to start are then short ones (24 sequences of up to 1096 tokens:
+// the scan 186 us as given, 168 so). The place is looked for bit by bit of the chunk
+// counts.
 __device__ __forceinline__ int longest_first(const PrefillArgs& a, int place, int& first_slot) {
   const int lane = threadIdx.x & 63, most = min((int)chunked_most(a.T, a.N, a.chunk_from), 64), group = place / most, base = 64 * group;
   first_slot = 0;
